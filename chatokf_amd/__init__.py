@@ -29,7 +29,8 @@ EXPORTS = (
     "okf_ctx_create", "okf_ctx_destroy", "okf_ctx_stream", "okf_ctx_reserve", "okf_row_bytes",
     "okf_gemv", "okf_gemv_silu", "okf_gemv_gate_up", "okf_ffn", "okf_silu_mul", "okf_gemm", "okf_gemm_tile", "okf_dequant_row",
     "okf_embed_batch", "okf_add_rmsnorm_batch", "okf_argmax_rows", "okf_argmax_rows_noalloc",
-    "okf_stream_read", "okf_parallel_begin",
+    "okf_stream_read", "okf_attn_prompt", "okf_attn_decode", "okf_kv_append", "okf_kv_read", "okf_kv_evict",
+    "okf_parallel_begin",
     "okf_parallel_end", "okf_sync", "okf_set_fault_rate", "okf_last_hip_error", "okf_strerror",
     "okf_gguf_open", "okf_gguf_close", "okf_gguf_tensor_count", "okf_gguf_tensor_at", "okf_gguf_find",
     "okf_gguf_kv_int", "okf_gguf_kv_double", "okf_gguf_kv_string", "okf_gguf_data", "okf_gguf_upload",
@@ -60,6 +61,29 @@ class OkfWeight(ctypes.Structure):
     ]
 
 
+class OkfAttn(ctypes.Structure):
+    """``okf_attn`` of include/okf_quant.h."""
+    _fields_ = (
+        [(n, ctypes.c_void_p) for n in ("q", "k", "v", "o")] + [("type", ctypes.c_int32)] +
+        [(n, ctypes.c_uint32) for n in ("heads", "kv_heads", "dim", "seqs", "n_q", "n_k")] +
+        [(n, ctypes.c_void_p) for n in ("q_start", "k_start")] +
+        [(n, ctypes.c_uint64) for n in ("q_stride", "k_stride", "v_stride", "o_stride", "q_head", "k_head", "v_head",
+                                        "o_head")] +
+        [("scale", ctypes.c_float), ("window", ctypes.c_uint32)])
+
+
+class OkfKVCache(ctypes.Structure):
+    """``okf_kv_cache`` of include/okf_quant.h."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] +
+                [(n, ctypes.c_uint32) for n in ("pages", "heads", "dim")])
+
+
+class OkfKVSeqs(ctypes.Structure):
+    """``okf_kv_seqs`` of include/okf_quant.h."""
+    _fields_ = [("pages", ctypes.c_void_p), ("len", ctypes.c_void_p), ("count", ctypes.c_uint32),
+                ("stride", ctypes.c_uint32)]
+
+
 class OkfError(RuntimeError):
     def __init__(self, status: int, what: str):
         self.status = status
@@ -79,6 +103,7 @@ def _lib():
         lib = ctypes.CDLL(LIB_PATH)
         vp, u32, u64, i32 = ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint64, ctypes.c_int32
         W = ctypes.POINTER(OkfWeight)
+        KC, KS = ctypes.POINTER(OkfKVCache), ctypes.POINTER(OkfKVSeqs)
         sig = {
             "okf_ctx_create": [ctypes.c_int, ctypes.POINTER(vp)],
             "okf_ctx_destroy": [vp],
@@ -98,6 +123,11 @@ def _lib():
             "okf_argmax_rows": [vp, vp, u32, u32, vp],
             "okf_argmax_rows_noalloc": [vp, vp, u32, u32, vp],
             "okf_stream_read": [vp, vp, ctypes.c_uint64, vp],
+            "okf_attn_prompt": [vp, ctypes.POINTER(OkfAttn)],
+            "okf_attn_decode": [vp, KC, KS, vp, vp, u32, u32, ctypes.c_float, u32, vp, vp, u64],
+            "okf_kv_append": [vp, KC, KS, vp, vp, i32, vp, u32, u64, u64],
+            "okf_kv_read": [vp, KC, KS, vp, vp, i32, vp, u32, u64, u64],
+            "okf_kv_evict": [vp, KC, KS, KC, KS, u32, u32, u32, vp, u64, vp, u64, vp],
             "okf_parallel_begin": [vp],
             "okf_parallel_end": [vp],
             "okf_sync": [vp],
@@ -155,6 +185,44 @@ class QuantTensor:
 
     def c(self) -> OkfWeight:
         return OkfWeight(_ptr(self.data), self.off, self.K, self.M, self.type)
+
+
+KV_BLOCK = 64  # OKF_KV_BLOCK
+
+
+class KVCache:
+    """``okf_kv_cache``: a paged KV cache of 8-bit codes in the caller's device
+    memory (torch tensors or raw pointers).  k int8 [pages][heads][64][dim], v
+    int8 [pages][heads][dim][64], scales fp32 [pages][heads]."""
+
+    def __init__(self, k, v, k_scale, v_scale, pages: int, heads: int, dim: int):
+        self.data = (k, v, k_scale, v_scale)
+        self.pages, self.heads, self.dim = int(pages), int(heads), int(dim)
+        self._c = OkfKVCache(_ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale), self.pages, self.heads, self.dim)
+
+    @classmethod
+    def new(cls, pages: int, heads: int, dim: int, device: int = 0) -> "KVCache":
+        """A cache in new torch tensors (nothing need be cleared)."""
+        import torch
+        dev = f"cuda:{device}"
+        codes = [torch.empty((pages, heads, KV_BLOCK, dim), dtype=torch.int8, device=dev),
+                 torch.empty((pages, heads, dim, KV_BLOCK), dtype=torch.int8, device=dev)]
+        return cls(*codes, *(torch.empty((pages, heads), device=dev) for _ in range(2)), pages, heads, dim)
+
+    def c(self) -> OkfKVCache:
+        return self._c
+
+
+class KVSeqs:
+    """``okf_kv_seqs``: the page table [count][stride] and lengths [count] (int32,
+    device memory) of sequences in a cache."""
+
+    def __init__(self, pages, lens, count: int, stride: int):
+        self.pages, self.lens, self.count, self.stride = pages, lens, int(count), int(stride)
+        self._c = OkfKVSeqs(_ptr(pages), _ptr(lens), self.count, self.stride)
+
+    def c(self) -> OkfKVSeqs:
+        return self._c
 
 
 class Enc:
@@ -294,6 +362,43 @@ class Enc:
         """okf_stream_read: out[0] ^= xor of the nbytes at p (a measurement kernel)."""
         self._check(self._lib.okf_stream_read(self.h, _ptr(p), int(nbytes), _ptr(out)), "okf_stream_read")
 
+    def attn_prompt(self, q, k, v, out, q_start, k_start, seqs: int, n_q: int, n_k: int, heads: int, kv_heads: int,
+                    dim: int, type: int = F32, scale: float = 1.0, window: int = 0, strides=(0, 0, 0, 0),
+                    head_strides=(0, 0, 0, 0)):
+        """okf_attn_prompt: causal attention over packed sequences; strides (of
+        rows) and head_strides of q, k, v, out in values, 0 for dense."""
+        a = OkfAttn(_ptr(q), _ptr(k), _ptr(v), _ptr(out), int(type), heads, kv_heads, dim, seqs, n_q, n_k,
+                    _ptr(q_start), _ptr(k_start), *strides, *head_strides, scale, window)
+        self._check(self._lib.okf_attn_prompt(self.h, ctypes.byref(a)), "okf_attn_prompt")
+
+    def attn_decode(self, cache: KVCache, seqs: KVSeqs, q, out, tokens: int, heads: int, scale: float,
+                    window: int = 0, w_in=None, w_out=None, w_stride: int = 0):
+        """okf_attn_decode: the last `tokens` tokens of each sequence attend to the
+        cache; with w_out the attention weight of each cached token is added up."""
+        self._check(self._lib.okf_attn_decode(self.h, ctypes.byref(cache.c()), ctypes.byref(seqs.c()), _ptr(q),
+                                              _ptr(out), tokens, heads, scale, window, _ptr(w_in), _ptr(w_out),
+                                              w_stride), "okf_attn_decode")
+
+    def kv_append(self, cache: KVCache, seqs: KVSeqs, k, v, start, n: int, type: int = F32, k_stride: int = 0,
+                  v_stride: int = 0):
+        """okf_kv_append: quantize n packed new tokens (start: each sequence's rows) into the cache."""
+        self._check(self._lib.okf_kv_append(self.h, ctypes.byref(cache.c()), ctypes.byref(seqs.c()), _ptr(k), _ptr(v),
+                                            int(type), _ptr(start), n, k_stride, v_stride), "okf_kv_append")
+
+    def kv_read(self, cache: KVCache, seqs: KVSeqs, k, v, start, n: int, type: int = F32, k_stride: int = 0,
+                v_stride: int = 0):
+        """okf_kv_read: the values of each sequence's last tokens, as packed rows."""
+        self._check(self._lib.okf_kv_read(self.h, ctypes.byref(cache.c()), ctypes.byref(seqs.c()), _ptr(k), _ptr(v),
+                                          int(type), _ptr(start), n, k_stride, v_stride), "okf_kv_read")
+
+    def kv_evict(self, src: KVCache, seqs: KVSeqs, dst: KVCache, to: KVSeqs, keep: int, sink: int, recent: int, w_in,
+                 w_in_stride: int, w_out, w_out_stride: int, kept):
+        """okf_kv_evict: cut each sequence to `keep` tokens a head, by accumulated attention weight."""
+        self._check(self._lib.okf_kv_evict(self.h, ctypes.byref(src.c()), ctypes.byref(seqs.c()),
+                                           ctypes.byref(dst.c()), ctypes.byref(to.c()), keep, sink, recent,
+                                           _ptr(w_in), w_in_stride, _ptr(w_out), w_out_stride, _ptr(kept)),
+                    "okf_kv_evict")
+
     def reserve(self, gemm_nk: int, argmax_n: int, argmax_rows: int):
         """okf_ctx_reserve: allocate the scratch now; later calls allocate nothing."""
         self._check(self._lib.okf_ctx_reserve(self.h, int(gemm_nk), int(argmax_n), int(argmax_rows)),
@@ -401,5 +506,5 @@ class GGUF:
 __all__ = [
     "Q8_0", "Q4_K", "IQ2_XXS", "Q2_0", "Q4_0", "IQ4_NL", "Q5_K", "Q6_K", "IQ4_XS", "IQ2_XS", "IQ2_S", "IQ3_XXS", "IQ3_S",
     "IQ1_S", "IQ1_M", "F32", "F16", "BF16", "Q2_K", "Q3_K", "NAMES", "BY_NAME", "block_elems", "row_bytes",
-    "QuantTensor", "Enc", "OkfError", "OkfWeight", "OkfGGUFTensor", "GGUF", "lib", "EXPORTS", "LIB_PATH",
+    "QuantTensor", "KVCache", "KVSeqs", "KV_BLOCK", "OkfAttn", "OkfKVCache", "OkfKVSeqs", "Enc", "OkfError", "OkfWeight", "OkfGGUFTensor", "GGUF", "lib", "EXPORTS", "LIB_PATH",
 ]

@@ -1,0 +1,173 @@
+// okf_attn.hip -- the C ABI of attention and the KV cache (include/okf_quant.h)
+// over okf_attn.h and okf_kv.h.
+#include "okf_impl.h"
+#include "okf_attn.h"
+
+namespace {
+
+using namespace okf;
+using namespace okf_impl;
+
+bool aligned4(const void *p) { return ((uintptr_t)p & 3) == 0; }
+
+bool attn_type(int32_t t) { return t == F32 || t == F16 || t == BF16; }
+
+// Runs f with a value of the element type t (attn_type).
+template <class Fn>
+void with_type(int32_t t, Fn f) {
+    if (t == F32) f(float{});
+    else if (t == F16) f(_Float16{});
+    else f(__bf16{});
+}
+
+bool good_dim(uint32_t d) { return d >= 16 && d <= 256 && d % 16 == 0; }
+
+int check_cache(const okf_kv_cache *c) {
+    if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) return OKF_E_ARG;
+    if (!c->pages || c->pages > 0x7FFFFFFFu || !c->heads || c->heads > 65535 || !good_dim(c->dim)) return OKF_E_SHAPE;
+    if (!aligned16(c->k) || !aligned16(c->v) || !aligned4(c->k_scale) || !aligned4(c->v_scale)) return OKF_E_SHAPE;
+    return OKF_OK;
+}
+
+int check_seqs(const okf_kv_seqs *s) {
+    if (!s || !s->pages || !s->len) return OKF_E_ARG;
+    if (!s->count || !s->stride || !aligned4(s->pages) || !aligned4(s->len)) return OKF_E_SHAPE;
+    return OKF_OK;
+}
+
+KvCache cache_of(const okf_kv_cache *c) { return {c->k, c->v, c->k_scale, c->v_scale, c->pages, c->heads, c->dim}; }
+KvSeqs seqs_of(const okf_kv_seqs *s) { return {s->pages, s->len, s->count, s->stride}; }
+
+// A row stride of 16-byte rows: `least` values when 0, else at least that and whole 16 bytes.
+bool row_stride(uint64_t &st, uint64_t least, uint32_t size) {
+    if (!st) st = least;
+    return st >= least && st <= (1ull << 40) && st * size % 16 == 0;
+}
+
+// Arguments that okf_kv_append and okf_kv_read share, and their grid: n rows of
+// `count` sequences touch at most n / 64 + 2 count page blocks.
+int check_rows(const okf_kv_cache *c, const okf_kv_seqs *s, const void *k, const void *v, int32_t type,
+               const int32_t *start, uint32_t n, uint64_t &ks, uint64_t &vs, dim3 &grid) {
+    int st = check_cache(c);
+    if (!st) st = check_seqs(s);
+    if (st) return st;
+    if (!start) return OKF_E_ARG;
+    if (!attn_type(type)) return OKF_E_TYPE;
+    const uint32_t size = type == F32 ? 4 : 2;
+    if (!n || n > 0x7FFFFFFFu || !aligned16(k) || !aligned16(v) || !aligned4(start)) return OKF_E_SHAPE;
+    const uint64_t row = (uint64_t)c->heads * c->dim;
+    if (!row_stride(ks, row, size) || !row_stride(vs, row, size)) return OKF_E_SHAPE;
+    const uint64_t items = n / KV_B + 3ull * s->count;
+    if (items > 0x7FFFFFFFull) return OKF_E_SHAPE;
+    grid = dim3((uint32_t)items, c->heads, 2);
+    return OKF_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int okf_attn_prompt(okf_ctx *c, const okf_attn *p) {
+    if (!p || !p->q || !p->k || !p->v || !p->o || !p->q_start || !p->k_start) return OKF_E_ARG;
+    if (!attn_type(p->type)) return OKF_E_TYPE;
+    if (!p->heads || !p->kv_heads || p->heads % p->kv_heads || p->heads > 65535 || !good_dim(p->dim)) return OKF_E_SHAPE;
+    if (!p->seqs || !p->n_q || !p->n_k || p->n_q > 0x7FFFFFFFu || p->n_k > 0x7FFFFFFFu) return OKF_E_SHAPE;
+    const uint32_t size = p->type == F32 ? 4 : 2;
+    AttnArgs a{p->q, p->k, p->v, p->o, p->heads, p->kv_heads, p->dim, p->seqs, p->n_q, p->n_k, p->q_start, p->k_start,
+               p->q_stride, p->k_stride, p->v_stride, p->o_stride, p->q_head, p->k_head, p->v_head, p->o_head,
+               p->scale, p->window};
+    // (rows may lie inside a head's plane, heads inside a row: either stride may be the larger)
+    const uint64_t least = p->dim;
+    if (!a.qs) a.qs = (uint64_t)p->heads * p->dim;
+    if (!a.os) a.os = (uint64_t)p->heads * p->dim;
+    if (!a.ks) a.ks = (uint64_t)p->kv_heads * p->dim;
+    if (!a.vs) a.vs = (uint64_t)p->kv_heads * p->dim;
+    for (uint64_t *s : {&a.qs, &a.ks, &a.vs, &a.os, &a.qh, &a.kh, &a.vh, &a.oh})
+        if (!row_stride(*s, least, size)) return OKF_E_SHAPE;
+    if (!aligned16(p->q) || !aligned16(p->k) || !aligned16(p->v) || !aligned16(p->o) || !aligned4(p->q_start) ||
+        !aligned4(p->k_start))
+        return OKF_E_SHAPE;
+    int st = begin(c);
+    if (st) return st;
+    with_type(p->type, [&](auto t) {
+        hipLaunchKernelGGL((attn_prompt_kernel<decltype(t)>), dim3(p->n_q, p->heads), dim3(AT_NT), 0, c->stream, a);
+    });
+    return finish(c);
+}
+
+int okf_attn_decode(okf_ctx *c, const okf_kv_cache *cache, const okf_kv_seqs *seqs, const float *q, float *o,
+                    uint32_t tokens, uint32_t heads, float scale, uint32_t window, const float *w_in, float *w_out,
+                    uint64_t w_stride) {
+    int st = check_cache(cache);
+    if (!st) st = check_seqs(seqs);
+    if (st) return st;
+    if (!q || !o || (w_in && !w_out)) return OKF_E_ARG;
+    if (!tokens || tokens > 65535 || !heads || heads % cache->heads || heads > 65535) return OKF_E_SHAPE;
+    if (!aligned16(q) || !aligned16(o) || !aligned4(w_in) || !aligned4(w_out)) return OKF_E_SHAPE;
+    if (w_out && w_stride < (uint64_t)seqs->stride * KV_B) return OKF_E_SHAPE;
+    if ((uint64_t)seqs->count * cache->heads > 0x7FFFFFFFull) return OKF_E_SHAPE;
+    if ((st = begin(c))) return st;
+    const DecArgs a{cache_of(cache), seqs_of(seqs), q, o, tokens, heads, scale, window, w_in, w_out, w_stride};
+    hipLaunchKernelGGL(attn_decode_kernel, dim3(seqs->count * cache->heads), dim3(AT_NT), 0, c->stream, a);
+    return finish(c);
+}
+
+int okf_kv_append(okf_ctx *c, const okf_kv_cache *cache, const okf_kv_seqs *seqs, const void *k, const void *v,
+                  int32_t type, const int32_t *start, uint32_t n, uint64_t k_stride, uint64_t v_stride) {
+    if (!k || !v) return OKF_E_ARG;
+    dim3 grid;
+    int st = check_rows(cache, seqs, k, v, type, start, n, k_stride, v_stride, grid);
+    if (st) return st;
+    if ((st = begin(c))) return st;
+    with_type(type, [&](auto t) {
+        using T = decltype(t);
+        hipLaunchKernelGGL((kv_append_kernel<T>), grid, dim3(KV_NT), 0, c->stream, cache_of(cache), seqs_of(seqs),
+                           (const T *)k, (const T *)v, start, n, k_stride, v_stride);
+    });
+    return finish(c);
+}
+
+int okf_kv_read(okf_ctx *c, const okf_kv_cache *cache, const okf_kv_seqs *seqs, void *k, void *v, int32_t type,
+                const int32_t *start, uint32_t n, uint64_t k_stride, uint64_t v_stride) {
+    if (!k && !v) return OKF_E_ARG;
+    dim3 grid;
+    int st = check_rows(cache, seqs, k, v, type, start, n, k_stride, v_stride, grid);
+    if (st) return st;
+    if ((st = begin(c))) return st;
+    with_type(type, [&](auto t) {
+        using T = decltype(t);
+        hipLaunchKernelGGL((kv_read_kernel<T>), grid, dim3(KV_NT), 0, c->stream, cache_of(cache), seqs_of(seqs),
+                           (T *)k, (T *)v, start, n, k_stride, v_stride);
+    });
+    return finish(c);
+}
+
+int okf_kv_evict(okf_ctx *c, const okf_kv_cache *src, const okf_kv_seqs *from, const okf_kv_cache *dst,
+                 const okf_kv_seqs *to, uint32_t keep, uint32_t sink, uint32_t recent, const float *w_in,
+                 uint64_t w_in_stride, float *w_out, uint64_t w_out_stride, int32_t *kept) {
+    int st = check_cache(src);
+    if (!st) st = check_seqs(from);
+    if (!st) st = check_cache(dst);
+    if (!st) st = check_seqs(to);
+    if (st) return st;
+    if (!w_in || !kept) return OKF_E_ARG;
+    if (src->heads != dst->heads || src->dim != dst->dim || from->count != to->count) return OKF_E_SHAPE;
+    if (!keep || keep > 0x7FFFFFFFu || (uint64_t)sink + recent > keep || keep > (uint64_t)to->stride * KV_B)
+        return OKF_E_SHAPE;
+    if (w_in_stride < (uint64_t)from->stride * KV_B || (w_out && w_out_stride < keep)) return OKF_E_SHAPE;
+    if (!aligned4(w_in) || !aligned4(w_out) || !aligned4(kept)) return OKF_E_SHAPE;
+    const uint64_t rows = (uint64_t)from->count * src->heads;
+    if (rows > 0x7FFFFFFFull) return OKF_E_SHAPE;
+    // (the second grid: sequences over y, in groups that fit it, and z)
+    const uint32_t group = std::min(from->count, 65535 / src->heads);
+    const uint32_t groups = (from->count + group - 1) / group;
+    if (groups > 65535) return OKF_E_SHAPE;
+    if ((st = begin(c))) return st;
+    hipLaunchKernelGGL(kv_select_kernel, dim3((uint32_t)rows), dim3(EV_NT), 0, c->stream, seqs_of(from), to->len,
+                       src->heads, keep, sink, recent, w_in, w_in_stride, w_out, w_out_stride, kept);
+    hipLaunchKernelGGL(kv_gather_kernel, dim3((keep + KV_B - 1) / KV_B, group * src->heads, groups), dim3(KV_NT), 0,
+                       c->stream, cache_of(src), seqs_of(from), cache_of(dst), seqs_of(to), keep, kept);
+    return finish(c);
+}
+
+}  // extern "C"

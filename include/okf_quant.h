@@ -239,6 +239,116 @@ int okf_stream_read(okf_ctx *ctx, const void *p, uint64_t bytes, uint32_t *out);
  * [0, M) is clamped to the nearest row. */
 int okf_embed_batch(okf_ctx *ctx, const okf_weight *w, const int32_t *ids, uint32_t N, float *out);
 
+/* ----------------------------------------------------------- attention --
+ * What stands between the projections of a decode step or a prompt: causal
+ * attention over a prompt, a paged KV cache of 8-bit codes, attention over
+ * that cache, and eviction from it.  The reference keeps its cache and
+ * attention in its engines; these entry points have layouts of their own.
+ * Head widths are multiples of 16 up to 256; query head h reads key / value
+ * head h / (heads / kv_heads).  Keys come with their positions already in
+ * them (rotated, where a model rotates). */
+
+/* Causal attention over packed sequences: o = softmax(scale q k^T) v.
+ * Sequence s has the query rows [q_start[s], q_start[s + 1]) and the key /
+ * value rows [k_start[s], k_start[s + 1]); its queries are its last rows, so
+ * that query i of nq stands at key nk - nq + i, sees the keys up to there and,
+ * with a window, only the last `window` of them.  A row that sees no key (nq
+ * > nk, or a score of -inf for all of them) gives 0; keys and values that a
+ * row does not see have no influence on it, NaN and infinities included.
+ * Starts that leave [0, n_q] / [0, n_k] or decrease are clamped.  Scores,
+ * sums and products are held in fp32; with f32 inputs the products keep
+ * fp32 precision, with f16 / bf16 the softmax weights are rounded to that
+ * type for the second product, and o once.  Scratch: none. */
+typedef struct {
+    const void *q, *k, *v;          /* rows of heads x dim / kv_heads x dim values */
+    void *o;                        /* n_q rows of heads x dim */
+    int32_t type;                   /* of q, k, v and o: OKF_TYPE_F32, _F16 or _BF16 */
+    uint32_t heads, kv_heads, dim;
+    uint32_t seqs, n_q, n_k;        /* sequences, query rows, key rows in all */
+    const int32_t *q_start, *k_start;   /* device memory, seqs + 1 each */
+    uint64_t q_stride, k_stride, v_stride, o_stride; /* values from a row to the next (0: dense) */
+    uint64_t q_head, k_head, v_head, o_head;         /* values from a head to the next (0: dim) */
+    float scale;
+    uint32_t window;                /* 0: none */
+} okf_attn;
+/* Pointers are 16-byte aligned and strides whole multiples of 16 bytes. */
+int okf_attn_prompt(okf_ctx *ctx, const okf_attn *a);
+
+/* A paged KV cache: a page holds OKF_KV_BLOCK tokens of every head, as int8
+ * codes with one fp32 scale for each page and head, for keys and values each
+ * (value = code * scale).
+ *   k[page][head][token][dim]
+ *   v[page][head][dim][slot], slot(t) = t % 16 / 4 * 16 + t / 16 * 4 + t % 4:
+ *     the order in which the matrix cores take a block's tokens
+ * Caller's device memory, k and v 16-byte aligned; nothing need be cleared. */
+#define OKF_KV_BLOCK 64
+typedef struct {
+    int8_t *k, *v;
+    float *k_scale, *v_scale;       /* [page][head] */
+    uint32_t pages, heads, dim;     /* heads: the kv heads */
+} okf_kv_cache;
+
+/* Sequences in a cache: token t of sequence s is token t % 64 of page
+ * pages[s * stride + t / 64].  An entry outside [0, cache.pages) holds no
+ * tokens: they are not attended to, read as 0, and what is appended there is
+ * dropped; so with tokens past stride * 64.  Sequences may share pages that
+ * none of them is appended to. */
+typedef struct {
+    const int32_t *pages;           /* device memory, [count][stride] */
+    int32_t *len;                   /* device memory, [count]: tokens held */
+    uint32_t count, stride;
+} okf_kv_seqs;
+
+/* Quantizes new tokens into the cache.  k and v: n rows of heads x dim values
+ * of `type` (row strides in values, 0: dense); sequence s gets the rows
+ * [start[s], start[s + 1]) as its last ones: len counts them already.  For
+ * each page and head: scale = max(old scale where the page held tokens of the
+ * sequence before, largest |x| / 127); codes held before are rounded to the
+ * larger scale (from the 64-bit product with the scales' quotient), new ones
+ * are x / scale rounded exactly, ties to even.  A NaN or infinity makes the
+ * page's scale of that head NaN: its tokens read as NaN until the page is
+ * begun anew. */
+int okf_kv_append(okf_ctx *ctx, const okf_kv_cache *cache, const okf_kv_seqs *seqs, const void *k, const void *v,
+                  int32_t type, const int32_t *start, uint32_t n, uint64_t k_stride, uint64_t v_stride);
+
+/* Reads values back: the last start[s + 1] - start[s] tokens of sequence s to
+ * the rows from start[s] of k and v (either may be NULL), code * scale rounded
+ * once to `type`: what okf_attn_prompt takes for a chunk behind a cached
+ * prefix.  Rows past the sequence's beginning are 0. */
+int okf_kv_read(okf_ctx *ctx, const okf_kv_cache *cache, const okf_kv_seqs *seqs, void *k, void *v, int32_t type,
+                const int32_t *start, uint32_t n, uint64_t k_stride, uint64_t v_stride);
+
+/* Attention of each sequence's last `tokens` tokens (one in a decode step,
+ * several in a verify pass) to the cache, which holds them already: query t
+ * stands at len - tokens + t and sees the tokens up to there, with a window
+ * only the last `window` of them; one that sees none gives 0.  q and o:
+ * fp32 [count][tokens][heads][dim], 16-byte aligned.  Codes enter the integer
+ * matrix cores as they are; queries and weights as 23-bit integers, so the
+ * result has fp32 precision.  With w_out, the attention weight that each
+ * token got is added up: w_out[s][head][t] = w_in[s][head][t] + the sum over
+ * the queries and the query heads of the kv head, t < len, rows of w_stride
+ * values; w_in NULL counts as 0, w_in = w_out adds in place.
+ * Scratch: the partial results of sequences split over workgroups, in the
+ * context's buffer (see okf_ctx_reserve); where it may not grow, fewer splits
+ * (the order of the fp32 sums changes). */
+int okf_attn_decode(okf_ctx *ctx, const okf_kv_cache *cache, const okf_kv_seqs *seqs, const float *q, float *o,
+                    uint32_t tokens, uint32_t heads, float scale, uint32_t window, const float *w_in, float *w_out,
+                    uint64_t w_stride);
+
+/* Cuts each sequence, per kv head, to `keep` tokens: its first `sink`, its
+ * last `recent`, and of those between the ones of the largest weight w_in
+ * (ties to the lower index; NaN lowest), in their order; a sequence of at most
+ * `keep` tokens stays whole.  The tokens go to the pages of `to`, which must
+ * be other ones than `from`'s (they may be of the same cache); to->len is
+ * written.  A new page's scale is the largest of its tokens' scales; codes
+ * under another scale are rounded (64-bit product with the scales' quotient).
+ * kept[s][head][keep]: the tokens' old indices, then -1.  w_out, if not NULL:
+ * their weights, in w_out[s][head][0 .. to->len).  sink + recent <= keep <=
+ * 64 to->stride; w rows as for okf_attn_decode. */
+int okf_kv_evict(okf_ctx *ctx, const okf_kv_cache *src, const okf_kv_seqs *from, const okf_kv_cache *dst,
+                 const okf_kv_seqs *to, uint32_t keep, uint32_t sink, uint32_t recent, const float *w_in,
+                 uint64_t w_in_stride, float *w_out, uint64_t w_out_stride, int32_t *kept);
+
 /* Waits for all work on the context's stream: the analogue of
  * commit + waitUntilCompleted (LLM/Base/MetalGates.swift:144-149).  Returns
  * OKF_E_HIP if a kernel failed. */
