@@ -1,5 +1,4 @@
-// okf_attn.h -- causal attention over packed prompts (okf_attn_prompt) and over
-// the paged 8-bit cache (okf_attn_decode).
+// okf_attn.h -- causal attention over packed prompts (okf_attn_prompt).
 #pragma once
 #include "okf_kv.h"
 
@@ -87,64 +86,6 @@ __global__ __launch_bounds__(AT_NT) void attn_prompt_kernel(AttnArgs a) {
         },
         [&](uint32_t j, uint32_t d) { return to_f32(v[j * a.vs + d]); }, m, l);
     if (tid < D) ((T *)a.o)[r * a.os + h * a.oh + tid] = (T)o;
-}
-
-struct DecArgs {
-    KvCache c;
-    KvSeqs s;
-    const float *q;
-    float *o;
-    uint32_t tokens, heads;
-    float scale;
-    uint32_t window;
-    const float *w_in;
-    float *w_out;
-    uint64_t wst;
-};
-
-__global__ __launch_bounds__(AT_NT) void attn_decode_kernel(DecArgs a) {
-    __shared__ float q[256], p[AT_NT], red[AT_NT / 64];
-    const uint32_t kh = blockIdx.x % a.c.heads, s = blockIdx.x / a.c.heads, tid = threadIdx.x, D = a.c.dim;
-    const uint32_t G = a.heads / a.c.heads, T = a.tokens;
-    const int64_t len = max(a.s.len[s], 0);
-    const uint32_t cap = (uint32_t)min(len, (int64_t)a.s.stride * KV_B);
-    const int32_t *pages = a.s.pages + (uint64_t)s * a.s.stride;
-    float *wo = a.w_out ? a.w_out + ((uint64_t)s * a.c.heads + kh) * a.wst : nullptr;
-    if (wo)
-        for (uint32_t j = tid; j < cap; j += AT_NT)
-            wo[j] = a.w_in ? a.w_in[((uint64_t)s * a.c.heads + kh) * a.wst + j] : 0.0f;
-    for (uint32_t r = 0; r < T * G; r++) {
-        const uint32_t t = r / G, h = kh * G + r % G;
-        const uint64_t at = (((uint64_t)s * T + t) * a.heads + h) * D;
-        __syncthreads();
-        if (tid < D) q[tid] = a.q[at + tid];
-        __syncthreads();
-        const uint32_t end = (uint32_t)max(len - T + t + 1, (int64_t)0), hi = min(end, cap);
-        const uint32_t lo = a.window && end > a.window ? end - a.window : 0;
-        auto key = [&](uint32_t j) {
-            const int32_t page = pages[j / KV_B];
-            if ((uint32_t)page >= a.c.pages) return -__builtin_inff();
-            const uint64_t ph = (uint64_t)page * a.c.heads + kh;
-            const int8_t *k = a.c.k + (ph * KV_B + j % KV_B) * D;
-            float x = 0;
-            for (uint32_t d = 0; d < D; d++) x += q[d] * (float)k[d];
-            return x * a.c.ks[ph] * a.scale;
-        };
-        float m, l;
-        const float o = at_row(
-            lo, hi, D, p, red, key,
-            [&](uint32_t j, uint32_t d) {
-                const int32_t page = pages[j / KV_B];
-                if ((uint32_t)page >= a.c.pages) return 0.0f;
-                const uint64_t ph = (uint64_t)page * a.c.heads + kh;
-                return (float)a.c.v[(ph * D + d) * KV_B + kv_slot(j % KV_B)] * a.c.vs[ph];
-            },
-            m, l);
-        if (tid < D) a.o[at + tid] = o;
-        if (wo && l != 0)
-            for (uint32_t j = lo / AT_NT * AT_NT + tid; j < hi; j += AT_NT)  // (a token stays with its thread)
-                if (j >= lo) wo[j] += expf(key(j) - m) / l;
-    }
 }
 
 }  // namespace okf

@@ -1,7 +1,8 @@
 // okf_attn.hip -- the C ABI of attention and the KV cache (include/okf_quant.h)
-// over okf_attn.h and okf_kv.h.
+// over okf_attn.h, okf_attn_dec.h and okf_kv.h.
 #include "okf_impl.h"
 #include "okf_attn.h"
+#include "okf_attn_dec.h"
 
 namespace {
 
@@ -63,6 +64,59 @@ int check_rows(const okf_kv_cache *c, const okf_kv_seqs *s, const void *k, const
     return OKF_OK;
 }
 
+// The splits of okf_attn_decode: how many page ranges each sequence and kv head
+// is cut into, so that the workgroups fill the CUs (as many at a time on each as the
+// kernel's registers leave room for: two for 16 rows of up to 128 dimensions or 32 of
+// up to 64, one past that), but no range of less than a page for each of a
+// workgroup's wavefronts; batches of ragged sequences get twice that, so that the
+// short ones' workgroups make room for the long ones'.  The partial results go to
+// the context's buffer; where it may not grow, as many splits as it holds.
+int plan_decode(okf_ctx *c, DecArgs &a) {
+    const uint64_t rows = (uint64_t)a.tokens * (a.heads / a.c.heads), rpb = rows > 16 ? 32 : 16;
+    a.rb = (uint32_t)((rows + rpb - 1) / rpb);
+    const uint64_t base = (uint64_t)a.s.count * a.c.heads * a.rb;
+    uint64_t want = (uint64_t)c->cus * (a.c.dim * rpb <= 2048 ? 2 : 1) * (a.s.count > 1 ? 2 : 1);
+    const uint64_t span = a.window ? std::min<uint64_t>(((uint64_t)a.window + a.tokens) / KV_B + 2, a.s.stride) : a.s.stride;
+    uint64_t splits = std::max<uint64_t>(1, std::min((want + base - 1) / base, (span + DEC_W - 1) / DEC_W));
+    auto bytes = [&](uint64_t n) {  // m and l, then partial outputs
+        return base * n * rpb * 2 * sizeof(float) + (n > 1 ? base * n * rpb * a.c.dim * sizeof(float) : 0);
+    };
+    if (splits > 1 || a.w_out) {
+        if (bytes(splits) > c->part_bytes && grow_part(c, bytes(splits), true) != OKF_OK) {
+            while (splits > 1 && bytes(splits) > c->part_bytes) splits--;
+            if (a.w_out && bytes(splits) > c->part_bytes) return OKF_E_SHAPE;
+        }
+    }
+    a.splits = (uint32_t)splits;
+    if (splits > 1 || a.w_out) {
+        a.ml = c->part;
+        a.part = c->part + base * splits * rpb * 2;
+    }
+    if ((base * splits + 8 * a.rb) > 0x7FFFFFFFull) return OKF_E_SHAPE;
+    return OKF_OK;
+}
+
+template <int KS, int NR>
+void launch_decode_n(okf_ctx *c, const DecArgs &a) {
+    static std::atomic<uint64_t> attr{0};
+    set_lds_attr(c, (const void *)attn_dec_kernel<KS, NR>, attr);
+    const uint32_t sh = a.s.count * a.c.heads;
+    const size_t lds = (size_t)DEC_W * 16 * NR * (a.c.dim + 4 + 2) * sizeof(float);
+    hipLaunchKernelGGL((attn_dec_kernel<KS, NR>), dim3((sh * a.splits + 7) / 8 * 8 * a.rb), dim3(DEC_NT), lds, c->stream, a);
+    if (a.splits > 1)
+        hipLaunchKernelGGL(attn_dec_join_kernel, dim3(sh * a.tokens * (a.heads / a.c.heads)), dim3(DEC_NT), 0, c->stream, a,
+                           16u * NR);
+    if (a.w_out) {
+        const uint32_t parts = std::max(1u, std::min(4 * c->cus / sh, (a.s.stride + DEC_W - 1) / DEC_W));
+        hipLaunchKernelGGL((attn_dec_weights_kernel<KS, NR>), dim3(sh * parts), dim3(DEC_NT), 0, c->stream, a, parts);
+    }
+}
+
+template <int KS>
+void launch_decode(okf_ctx *c, const DecArgs &a, bool two) {
+    two ? launch_decode_n<KS, 2>(c, a) : launch_decode_n<KS, 1>(c, a);
+}
+
 }  // namespace
 
 extern "C" {
@@ -105,10 +159,19 @@ int okf_attn_decode(okf_ctx *c, const okf_kv_cache *cache, const okf_kv_seqs *se
     if (!tokens || tokens > 65535 || !heads || heads % cache->heads || heads > 65535) return OKF_E_SHAPE;
     if (!aligned16(q) || !aligned16(o) || !aligned4(w_in) || !aligned4(w_out)) return OKF_E_SHAPE;
     if (w_out && w_stride < (uint64_t)seqs->stride * KV_B) return OKF_E_SHAPE;
-    if ((uint64_t)seqs->count * cache->heads > 0x7FFFFFFFull) return OKF_E_SHAPE;
+    const uint64_t sh = (uint64_t)seqs->count * cache->heads, rows = (uint64_t)tokens * (heads / cache->heads);
+    if (sh * rows > 0x3FFFFFFFull) return OKF_E_SHAPE;
     if ((st = begin(c))) return st;
-    const DecArgs a{cache_of(cache), seqs_of(seqs), q, o, tokens, heads, scale, window, w_in, w_out, w_stride};
-    hipLaunchKernelGGL(attn_decode_kernel, dim3(seqs->count * cache->heads), dim3(AT_NT), 0, c->stream, a);
+    DecArgs a{cache_of(cache), seqs_of(seqs), q, o, tokens, heads, scale, window, w_in, w_out, w_stride, 1, 1,
+              nullptr, nullptr};
+    if ((st = plan_decode(c, a))) return st;
+    if (a.ml) note_capture(c, false, true, false);
+    switch ((cache->dim + 63) / 64) {
+    case 1: launch_decode<1>(c, a, rows > 16); break;
+    case 2: launch_decode<2>(c, a, rows > 16); break;
+    case 3: launch_decode<3>(c, a, rows > 16); break;
+    default: launch_decode<4>(c, a, rows > 16); break;
+    }
     return finish(c);
 }
 

@@ -1,0 +1,457 @@
+// okf_attn_dec.h -- attention of a sequence's last tokens to the paged 8-bit
+// cache (okf_attn_decode) on the integer matrix cores.
+//
+// Arithmetic.  A cached key is code * scale, so q k = scale_k f (Q code) with
+// Q = rint(q / f), f a power of two for each query row such that |Q| < 2^23:
+// three signed byte digits Q = Q2 2^16 + Q1 2^8 + Q0, each a column operand of
+// v_mfma_i32_16x16x64_i8 against the codes as they lie in memory.  Their sums
+// are exact in 32 bits ((Q1 code << 8) + Q0 code too), so a score's roundings
+// are Q's (2^-24 of the row's largest) and a few in fp32.  The softmax weights p
+// <= 1 (of the running maximum) become P = rint(p (2^23 - 2^15 - 2^7 - 1)) the
+// same way for the product with the value codes.  No code is ever unpacked.
+//
+// Layout.  A wavefront takes one page (64 tokens) at a time and 16 NR query rows
+// (row = query token * group + query head of the group).  Scores: A = 16 tokens
+// x 64 dimensions of K, B = a digit plane of the queries; a lane then holds,
+// for the query row lane % 16, tokens 16 t + 4 (lane / 16) + i.  Values: A = 16
+// dimensions x the page's 64 tokens, B = a digit plane of P, whose 16 bytes a lane
+// are just the tokens whose scores it holds, in the order that kv_slot gives
+// the value rows: no exchange between lanes, and no LDS, until the wavefronts
+// of a workgroup join their results at the end.
+#pragma once
+#include "okf_attn.h"
+#include "okf_ffn_mfma.h"
+
+namespace okf {
+
+constexpr uint32_t DEC_NT = 256, DEC_W = DEC_NT / 64;
+constexpr float DEC_P = 8355711.0f;      // 0x7F7F7F: the largest 3-digit number with signed byte digits
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct DecArgs {
+    KvCache c;
+    KvSeqs s;
+    const float *q;
+    float *o;
+    uint32_t tokens, heads;
+    float scale;
+    uint32_t window;
+    const float *w_in;
+    float *w_out;
+    uint64_t wst;
+    uint32_t splits, rb;   // page ranges a sequence; blocks of 16 NR query rows
+    float *part, *ml;      // [row block][split][16 NR][dim], [row block][split][16 NR][2]
+};
+
+// Four integers + 0x808080 -> the dwords of their three digit planes.
+__device__ __forceinline__ void dec_digits(uint32_t a, uint32_t b, uint32_t c, uint32_t d, int &p0, int &p1, int &p2) {
+    const uint32_t ab = perm(b, a, 0x05010400u), cd = perm(d, c, 0x05010400u);  // a0 b0 a1 b1
+    const uint32_t ah = perm(b, a, 0x0C0C0602u), ch = perm(d, c, 0x0C0C0602u);  // a2 b2
+    p0 = (int)(perm(cd, ab, 0x05040100u) ^ 0x80808080u);
+    p1 = (int)(perm(cd, ab, 0x07060302u) ^ 0x80808080u);
+    p2 = (int)(perm(ch, ah, 0x05040100u) ^ 0x80808080u);
+}
+
+// A block of 16 NR query rows of a sequence and kv head, as the B operands.
+template <int KS, int NR>
+struct DecQuery {
+    int32x4 d[NR][3][KS];
+    float f[NR];                // score of one unit of Q code, times log2 e
+    uint32_t hi[NR], lo[NR];
+    uint32_t hi_min, hi_max, lo_min, lo_max;   // over the workgroup's rows
+
+    __device__ __forceinline__ void load(const DecArgs &a, uint32_t s, uint32_t kh, uint32_t rb) {
+        const uint32_t lane = threadIdx.x & 63, g4 = lane >> 4, D = a.c.dim;
+        const uint32_t G = a.heads / a.c.heads, rows = a.tokens * G;
+        const int64_t len = max(a.s.len[s], 0);
+        const uint32_t cap = (uint32_t)min(len, (int64_t)a.s.stride * KV_B);
+        auto see = [&](uint32_t t, uint32_t &h, uint32_t &l) {
+            const int64_t end = max(len - a.tokens + t + 1, (int64_t)0);
+            h = (uint32_t)min(end, (int64_t)cap);
+            l = a.window && end > a.window ? (uint32_t)(end - a.window) : 0;
+        };
+        const uint32_t r0 = rb * 16 * NR, r1 = min(r0 + 16 * NR, rows) - 1;
+        see(r0 / G, hi_min, lo_min);
+        see(r1 / G, hi_max, lo_max);
+#pragma unroll
+        for (int n = 0; n < NR; n++) {
+            const uint32_t r = min(r0 + 16 * n + (lane & 15), r1), t = r / G, h = kh * G + r % G;
+            see(t, hi[n], lo[n]);
+            const float *q = a.q + (((uint64_t)s * a.tokens + t) * a.heads + h) * D;
+            floatx4 x[KS][4];
+            float m = 0, bad = 0;
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t d = 64 * k + 16 * g4;
+                    x[k][i] = d < D ? *(const floatx4 *)(q + d + 4 * i) : floatx4{0, 0, 0, 0};
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        m = fmaxf(m, fabsf(x[k][i][j]));
+                        bad = fmaf(x[k][i][j], 0.0f, bad);  // NaN for an infinity or NaN
+                    }
+                }
+            m = fmaxf(m, __shfl_xor(m, 16));
+            m = fmaxf(m, __shfl_xor(m, 32));
+            bad += __shfl_xor(bad, 16);
+            bad += __shfl_xor(bad, 32);
+            // m = c 2^e, c < 1: 2^(23 - e) where c 2^23 fits three digits
+            int e = __builtin_amdgcn_frexp_expf(m);
+            e = max(min(e + (__builtin_amdgcn_ldexpf(m, 23 - e) > DEC_P), 127), -100);
+            const float up = __builtin_amdgcn_ldexpf(1.0f, 23 - e);
+            f[n] = (__builtin_amdgcn_ldexpf(a.scale, e - 23) + bad) * LOG2E;
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    uint32_t y[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) y[j] = (uint32_t)(__float2int_rn(x[k][i][j] * up) + 0x808080);
+                    int p0, p1, p2;
+                    dec_digits(y[0], y[1], y[2], y[3], p0, p1, p2);
+                    d[n][0][k][i] = p0;
+                    d[n][1][k][i] = p1;
+                    d[n][2][k][i] = p2;
+                }
+            }
+        }
+    }
+};
+
+// The keys of a page as the A operand: tile t, dimensions 64 k + 16 (lane / 16) ..
+template <int KS>
+__device__ __forceinline__ void dec_load_k(int32x4 (&kk)[4][KS], const int8_t *page, uint32_t D) {
+    const uint32_t lane = threadIdx.x & 63;
+    const int8_t *p = page + (lane & 15) * D;
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int k = 0; k < KS; k++)  // (past the end: bytes of the row that meet zero digits)
+            kk[t][k] = *(const int32x4 *)(p + 16 * t * D + min(64 * k + 16 * (lane >> 4), D - 16));
+}
+
+// Scores of a page in units of log2, masked where the page is not wholly visible.
+template <int KS, int NR>
+__device__ __forceinline__ void dec_scores(float (&s)[NR][16], const int32x4 (&kk)[4][KS], const DecQuery<KS, NR> &q,
+                                           float ks, uint32_t j0) {
+    const uint32_t g4 = (threadIdx.x & 63) >> 4;
+    const bool whole = j0 + KV_B <= q.hi_min && j0 >= q.lo_max;
+#pragma unroll
+    for (int n = 0; n < NR; n++) {
+        const float f = q.f[n] * ks;
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            int32x4 c0 = {0, 0, 0, 0}, c1 = c0, c2 = c0;
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                c0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kk[t][k], q.d[n][0][k], c0, 0, 0, 0);
+                c1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kk[t][k], q.d[n][1][k], c1, 0, 0, 0);
+                c2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kk[t][k], q.d[n][2][k], c2, 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                s[n][4 * t + i] = fmaf((float)c2[i], 65536.0f, (float)((c1[i] << 8) + c0[i])) * f;
+        }
+        if (!whole) {
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t j = j0 + 16 * t + 4 * g4 + i;
+                    if (j < q.lo[n] || j >= q.hi[n]) s[n][4 * t + i] = -__builtin_inff();
+                }
+        }
+    }
+}
+
+// The pages that the splits share out: those that some row of the block sees.
+__device__ __forceinline__ uint2 dec_pages(uint32_t lo_min, uint32_t hi_max) {
+    return {lo_min / KV_B, (hi_max + KV_B - 1) / KV_B};
+}
+__device__ __forceinline__ uint32_t dec_chunk(uint2 pg, uint32_t splits) {
+    return pg.y > pg.x ? (pg.y - pg.x + splits - 1) / splits : 0;
+}
+
+// Grid: (row block, split, kv head, sequence) in one dimension, the row block
+// slowest: blocks that read the same pages lie a multiple of 8 apart.
+struct DecAt {
+    uint32_t s, kh, split, rb;
+    bool ok;
+};
+__device__ __forceinline__ DecAt dec_at(const DecArgs &a, uint32_t id) {
+    const uint32_t per = (a.s.count * a.c.heads * a.splits + 7) / 8 * 8, rb = id / per, i = id % per;
+    const uint32_t sh = i / a.splits;
+    return {sh / a.c.heads, sh % a.c.heads, i % a.splits, rb, sh < a.s.count * a.c.heads};
+}
+
+template <int KS, int NR>
+__global__ __launch_bounds__(DEC_NT, KS * NR <= 2 ? 2 : 1) void attn_dec_kernel(DecArgs a) {
+    extern __shared__ __align__(16) float dec_lds[];  // [wave][16 NR][dim + 4], then m and l [wave][16 NR]
+    float *const lds = dec_lds;
+    const DecAt at = dec_at(a, blockIdx.x);
+    if (!at.ok) return;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, D = a.c.dim, g4 = lane >> 4;
+    DecQuery<KS, NR> q;
+    q.load(a, at.s, at.kh, at.rb);
+    const uint2 pg = dec_pages(q.lo_min, q.hi_max);
+    const uint32_t chunk = dec_chunk(pg, a.splits);
+    const uint32_t p0 = pg.x + at.split * chunk, p1 = min(p0 + chunk, pg.y);
+    if (a.splits > 1 && p0 >= p1) return;  // (the joining kernel knows)
+    floatx4 o[NR][4 * KS] = {};
+    float m[NR], l[NR];
+#pragma unroll
+    for (int n = 0; n < NR; n++) m[n] = -__builtin_inff(), l[n] = 0;
+    const int32_t *pages = a.s.pages + (uint64_t)at.s * a.s.stride;
+    const uint64_t pbytes = (uint64_t)KV_B * D;
+    for (uint32_t b = p0 + wave; b < p1; b += 64 * DEC_W) {
+        // page ids and scales of this wavefront's next 64 pages, one a lane
+        const uint32_t mine = b + lane * DEC_W;
+        const int32_t id = mine < p1 ? pages[mine] : -1;
+        const bool have = (uint32_t)id < a.c.pages;
+        const uint64_t ph = have ? (uint64_t)id * a.c.heads + at.kh : 0;
+        const float lks = have ? a.c.ks[ph] : 0, lvs = have ? a.c.vs[ph] : 0;
+        uint64_t todo = __ballot(have);
+        if (!todo) continue;
+        int at_lane = __ffsll((unsigned long long)todo) - 1;
+        auto base = [&](int ln) {
+            const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)ph, ln), hi = __builtin_amdgcn_readlane((uint32_t)(ph >> 32), ln);
+            return (((uint64_t)hi << 32) | lo) * pbytes;
+        };
+        int32x4 kk[4][KS];
+        uint64_t off = base(at_lane);
+        dec_load_k<KS>(kk, a.c.k + off, D);
+        while (todo) {
+            const uint32_t j0 = (b + at_lane * DEC_W) * KV_B;
+            const float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lks), at_lane));
+            const float vs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lvs), at_lane));
+            int32x4 vv[4 * KS];
+            const int8_t *vp = a.c.v + off + (lane & 15) * KV_B + g4 * 16;
+#pragma unroll
+            for (int d = 0; d < 4 * KS; d++)
+                if (16u * d < D) vv[d] = *(const int32x4 *)(vp + d * 1024);
+            float s[NR][16];
+            dec_scores<KS, NR>(s, kk, q, ks, j0);
+            todo &= todo - 1;
+            if (todo) {
+                at_lane = __ffsll((unsigned long long)todo) - 1;
+                off = base(at_lane);
+                dec_load_k<KS>(kk, a.c.k + off, D);
+            }
+#pragma unroll
+            for (int n = 0; n < NR; n++) {
+                float x = s[n][0];
+#pragma unroll
+                for (int i = 1; i < 16; i++) x = fmaxf(x, s[n][i]);
+                x = fmaxf(x, __shfl_xor(x, 16));
+                x = fmaxf(x, __shfl_xor(x, 32));
+                const float nm = fmaxf(m[n], x), ref = nm == -__builtin_inff() ? 0.0f : nm;
+                if (__ballot(nm > m[n])) {
+                    const float f = __builtin_amdgcn_exp2f(m[n] - ref);
+                    l[n] *= f;
+#pragma unroll
+                    for (int d = 0; d < 4 * KS; d++) o[n][d] *= f;
+                }
+                m[n] = nm;
+                int32x4 pd[3];
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    uint32_t y[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float p = __builtin_amdgcn_exp2f(s[n][4 * t + i] - ref);
+                        l[n] += p;
+                        // (2^23 + P: P's rounding is the addition's, its digits the low three bytes)
+                        y[i] = __float_as_uint(fmaf(p, DEC_P, 8388608.0f)) + 0x808080u;
+                    }
+                    int d0, d1, d2;
+                    dec_digits(y[0], y[1], y[2], y[3], d0, d1, d2);
+                    pd[0][t] = d0, pd[1][t] = d1, pd[2][t] = d2;
+                }
+                // (a row that sees nothing of the page takes nothing from it, a NaN scale neither)
+                const float f = j0 < q.hi[n] && j0 + KV_B > q.lo[n] ? vs : 0.0f;
+#pragma unroll
+                for (int d = 0; d < 4 * KS; d++)
+                    if (16u * d < D) {
+                        const int32x4 z = {0, 0, 0, 0};
+                        const int32x4 c0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(vv[d], pd[0], z, 0, 0, 0);
+                        const int32x4 c1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(vv[d], pd[1], z, 0, 0, 0);
+                        const int32x4 c2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(vv[d], pd[2], z, 0, 0, 0);
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            o[n][d][i] += fmaf((float)c2[i], 65536.0f, (float)((c1[i] << 8) + c0[i])) * f;
+                    }
+            }
+        }
+    }
+    // the wavefronts' results joined
+    const uint32_t row = D + 4;
+    float *lm = lds + DEC_W * 16 * NR * row;
+#pragma unroll
+    for (int n = 0; n < NR; n++) {
+        l[n] += __shfl_xor(l[n], 16);
+        l[n] += __shfl_xor(l[n], 32);
+        if (lane < 16) {
+            lm[(wave * NR + n) * 32 + lane] = m[n];
+            lm[(wave * NR + n) * 32 + 16 + lane] = l[n];
+        }
+        float *p = lds + ((wave * NR + n) * 16 + (lane & 15)) * row + 4 * g4;
+#pragma unroll
+        for (int d = 0; d < 4 * KS; d++)
+            if (16u * d < D) *(floatx4 *)(p + 16 * d) = o[n][d];
+    }
+    __syncthreads();
+    const uint32_t G = a.heads / a.c.heads, rows = min(a.tokens * G - at.rb * 16 * NR, 16u * NR);
+    const uint64_t seg = ((uint64_t)at.rb * a.s.count * a.c.heads + at.s * a.c.heads + at.kh) * a.splits + at.split;
+    for (uint32_t e = threadIdx.x; e < rows * (D / 4); e += DEC_NT) {
+        const uint32_t r = e / (D / 4), d = e % (D / 4) * 4, n = r / 16;
+        float top = -__builtin_inff();
+#pragma unroll
+        for (uint32_t w = 0; w < DEC_W; w++) top = fmaxf(top, lm[(w * NR + n) * 32 + r % 16]);
+        const float ref = top == -__builtin_inff() ? 0.0f : top;
+        floatx4 sum = {0, 0, 0, 0};
+        float ls = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < DEC_W; w++) {
+            const float f = __builtin_amdgcn_exp2f(lm[(w * NR + n) * 32 + r % 16] - ref);
+            sum += *(const floatx4 *)(lds + ((w * NR + n) * 16 + r % 16) * row + d) * f;
+            ls += lm[(w * NR + n) * 32 + 16 + r % 16] * f;
+        }
+        if (a.splits > 1 || a.ml) {
+            if (d == 0) {
+                a.ml[(seg * 16 * NR + r) * 2] = top;
+                a.ml[(seg * 16 * NR + r) * 2 + 1] = ls;
+            }
+        }
+        if (a.splits > 1) {
+            *(floatx4 *)(a.part + (seg * 16 * NR + r) * D + d) = sum;
+        } else {
+            const uint32_t rr = at.rb * 16 * NR + r;
+            float *out = a.o + (((uint64_t)at.s * a.tokens + rr / G) * a.heads + at.kh * G + rr % G) * D + d;
+            *(floatx4 *)out = ls != 0 ? sum * (1.0f / (ls * DEC_P)) : floatx4{0, 0, 0, 0};
+        }
+    }
+}
+
+// Visible pages of a block of rows, as its first and last row see them.
+__device__ __forceinline__ uint2 dec_block_pages(const DecArgs &a, uint32_t s, uint32_t r0, uint32_t r1) {
+    const uint32_t G = a.heads / a.c.heads;
+    const int64_t len = max(a.s.len[s], 0);
+    const uint32_t cap = (uint32_t)min(len, (int64_t)a.s.stride * KV_B);
+    const int64_t e0 = max(len - a.tokens + r0 / G + 1, (int64_t)0), e1 = max(len - a.tokens + r1 / G + 1, (int64_t)0);
+    return dec_pages(a.window && e0 > a.window ? (uint32_t)(e0 - a.window) : 0, (uint32_t)min(e1, (int64_t)cap));
+}
+
+// Joins the splits: one workgroup a query row (query token and head); threads
+// take four dimensions of every (1024 / dim)-th split each.
+__global__ __launch_bounds__(DEC_NT) void attn_dec_join_kernel(DecArgs a, uint32_t rpb) {
+    __shared__ __align__(16) float acc[DEC_NT * 4];
+    const uint32_t G = a.heads / a.c.heads, rows = a.tokens * G, D = a.c.dim, tid = threadIdx.x;
+    const uint32_t r = blockIdx.x % rows, sh = blockIdx.x / rows, s = sh / a.c.heads, kh = sh % a.c.heads;
+    const uint32_t rb = r / rpb, r0 = rb * rpb;
+    const uint2 pg = dec_block_pages(a, s, r0, min(r0 + rpb, rows) - 1);
+    const uint32_t chunk = dec_chunk(pg, a.splits), ns = chunk ? (pg.y - pg.x + chunk - 1) / chunk : 0;
+    const uint64_t seg = ((uint64_t)rb * a.s.count * a.c.heads + sh) * a.splits;
+    const float *ml = a.ml + (seg * rpb + (r - r0)) * 2;
+    const uint64_t step = (uint64_t)rpb * 2;
+    float top = -__builtin_inff();
+    for (uint32_t i = 0; i < ns; i++) top = fmaxf(top, ml[i * step]);
+    const float ref = top == -__builtin_inff() ? 0.0f : top;
+    const uint32_t q4 = D / 4, groups = DEC_NT / q4, g = tid / q4, d = tid % q4 * 4;
+    floatx4 sum = {0, 0, 0, 0};
+    float ls = 0;
+    if (g < groups)
+        for (uint32_t i = g; i < ns; i += groups) {
+            const float f = __builtin_amdgcn_exp2f(ml[i * step] - ref);
+            ls += ml[i * step + 1] * f;
+            sum += *(const floatx4 *)(a.part + ((seg + i) * rpb + (r - r0)) * D + d) * f;
+        }
+    *(floatx4 *)(acc + tid * 4) = sum;
+    __syncthreads();
+    __shared__ float lsum[DEC_NT];
+    lsum[tid] = g < groups ? ls : 0;
+    __syncthreads();
+    if (tid < q4) {
+        for (uint32_t i = 1; i < groups; i++) {
+            sum += *(const floatx4 *)(acc + (i * q4 + tid) * 4);
+            ls += lsum[i * q4 + tid];
+        }
+        float *out = a.o + (((uint64_t)s * a.tokens + r / G) * a.heads + kh * G + r % G) * D + d;
+        *(floatx4 *)out = ls != 0 ? sum * (1.0f / (ls * DEC_P)) : floatx4{0, 0, 0, 0};
+    }
+}
+
+// Accumulated attention weights: a wavefront a page, the scores computed again
+// from the keys, for every block of query rows.  (Stored scores would be 8 bytes a
+// token and query row, and scratch of the cache's capacity.)
+template <int KS, int NR>
+__global__ __launch_bounds__(DEC_NT, KS <= 2 ? 2 : 1) void attn_dec_weights_kernel(DecArgs a, uint32_t parts) {
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, D = a.c.dim, g4 = lane >> 4;
+    const uint32_t sh = blockIdx.x / parts, s = sh / a.c.heads, kh = sh % a.c.heads, part = blockIdx.x % parts;
+    const uint32_t cap = (uint32_t)min((uint64_t)max(a.s.len[s], 0), (uint64_t)a.s.stride * KV_B);
+    const uint32_t np = (cap + KV_B - 1) / KV_B, chunk = (np + parts - 1) / parts;
+    const uint32_t rows = a.tokens * (a.heads / a.c.heads);
+    const int32_t *pages = a.s.pages + (uint64_t)s * a.s.stride;
+    const float *wi = a.w_in ? a.w_in + (uint64_t)sh * a.wst : nullptr;
+    float *wo = a.w_out + (uint64_t)sh * a.wst;
+    for (uint32_t rb = 0; rb < a.rb; rb++) {
+        DecQuery<KS, NR> q;
+        q.load(a, s, kh, rb);
+        // maximum and sum over the splits, for this lane's rows
+        const uint2 pg = dec_pages(q.lo_min, q.hi_max);
+        const uint32_t ch = dec_chunk(pg, a.splits), ns = ch ? (pg.y - pg.x + ch - 1) / ch : 0;
+        const uint64_t seg = ((uint64_t)rb * a.s.count * a.c.heads + sh) * a.splits;
+        float ref[NR], inv[NR];
+#pragma unroll
+        for (int n = 0; n < NR; n++) {
+            const bool valid = rb * 16 * NR + 16 * n + (lane & 15) < rows;
+            const float *ml = a.ml + (seg * 16 * NR + 16 * n + (lane & 15)) * 2;
+            float top = -__builtin_inff(), ls = 0;
+            if (valid)
+                for (uint32_t i = g4; i < ns; i += 4) top = fmaxf(top, ml[(uint64_t)i * 32 * NR]);
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            ref[n] = top == -__builtin_inff() ? 0.0f : top;
+            if (valid)
+                for (uint32_t i = g4; i < ns; i += 4)
+                    ls += ml[(uint64_t)i * 32 * NR + 1] * __builtin_amdgcn_exp2f(ml[(uint64_t)i * 32 * NR] - ref[n]);
+            ls += __shfl_xor(ls, 16);
+            ls += __shfl_xor(ls, 32);
+            inv[n] = valid && ls != 0 ? 1.0f / ls : 0.0f;
+        }
+        for (uint32_t p = part * chunk + wave; p < min((part + 1) * chunk, np); p += DEC_W) {
+            const uint32_t j0 = p * KV_B;
+            const int32_t id = pages[p];
+            const uint32_t j = j0 + lane;
+            float w = 0;
+            if ((uint32_t)id < a.c.pages && j0 < q.hi_max && j0 + KV_B > q.lo_min) {
+                const uint64_t ph = (uint64_t)id * a.c.heads + kh;
+                int32x4 kk[4][KS];
+                dec_load_k<KS>(kk, a.c.k + ph * KV_B * D, D);
+                float sc[NR][16], sum[16];
+                dec_scores<KS, NR>(sc, kk, q, a.c.ks[ph], j0);
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    sum[i] = 0;
+#pragma unroll
+                    for (int n = 0; n < NR; n++) {
+                        const float e = __builtin_amdgcn_exp2f(sc[n][i] - ref[n]) * inv[n];
+                        // (unseen tokens get nothing of a row whose sum is NaN)
+                        sum[i] += rb * 16 * NR + 16 * n + (lane & 15) < rows && sc[n][i] != -__builtin_inff() ? e : 0.0f;
+                    }
+#pragma unroll
+                    for (int x = 1; x < 16; x <<= 1) sum[i] += __shfl_xor(sum[i], x);
+                }
+                // token lane = 16 t + 4 g + i is held by lanes of group g, at 4 t + i
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const float v = __shfl(sum[i], (lane >> 2 & 3) * 16);
+                    if ((lane >> 4) == i / 4 && (lane & 3) == i % 4) w = v;
+                }
+            }
+            if (j < cap) wo[j] = (rb ? wo[j] : wi ? wi[j] : 0.0f) + w;
+        }
+    }
+}
+
+}  // namespace okf
