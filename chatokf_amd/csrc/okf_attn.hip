@@ -64,6 +64,13 @@ int check_rows(const okf_kv_cache *c, const okf_kv_seqs *s, const void *k, const
     return OKF_OK;
 }
 
+template <class T, int DP, bool FULL>
+void launch_prompt(okf_ctx *c, const AttnArgs &a) {
+    static std::atomic<uint64_t> attr{0};
+    set_lds_attr(c, (const void *)attn_prompt_kernel<T, DP, FULL>, attr);
+    hipLaunchKernelGGL((attn_prompt_kernel<T, DP, FULL>), dim3(a.tiles * a.heads), dim3(AT_NT), (at_lds<T, DP>()), c->stream, a);
+}
+
 // The splits of okf_attn_decode: how many page ranges each sequence and kv head
 // is cut into, so that the workgroups fill the CUs (as many at a time on each as the
 // kernel's registers leave room for: two for 16 rows of up to 128 dimensions or 32 of
@@ -129,7 +136,7 @@ int okf_attn_prompt(okf_ctx *c, const okf_attn *p) {
     const uint32_t size = p->type == F32 ? 4 : 2;
     AttnArgs a{p->q, p->k, p->v, p->o, p->heads, p->kv_heads, p->dim, p->seqs, p->n_q, p->n_k, p->q_start, p->k_start,
                p->q_stride, p->k_stride, p->v_stride, p->o_stride, p->q_head, p->k_head, p->v_head, p->o_head,
-               p->scale, p->window};
+               p->scale, p->window, 0};
     // (rows may lie inside a head's plane, heads inside a row: either stride may be the larger)
     const uint64_t least = p->dim;
     if (!a.qs) a.qs = (uint64_t)p->heads * p->dim;
@@ -138,13 +145,21 @@ int okf_attn_prompt(okf_ctx *c, const okf_attn *p) {
     if (!a.vs) a.vs = (uint64_t)p->kv_heads * p->dim;
     for (uint64_t *s : {&a.qs, &a.ks, &a.vs, &a.os, &a.qh, &a.kh, &a.vh, &a.oh})
         if (!row_stride(*s, least, size)) return OKF_E_SHAPE;
+    if (a.ks > 1u << 23 || a.vs > 1u << 23) return OKF_E_SHAPE;  // (a tile's rows are addressed by 32-bit offsets)
     if (!aligned16(p->q) || !aligned16(p->k) || !aligned16(p->v) || !aligned16(p->o) || !aligned4(p->q_start) ||
         !aligned4(p->k_start))
         return OKF_E_SHAPE;
     int st = begin(c);
     if (st) return st;
+    // (sequences' tiles: at most n_q / 128 and one each; never more than the rows)
+    const uint64_t tiles = std::min<uint64_t>((uint64_t)p->n_q / AT_BM + p->seqs, p->n_q);
+    if (tiles * p->heads > 0x7FFFFFFFull) return OKF_E_SHAPE;
+    a.tiles = (uint32_t)tiles;
     with_type(p->type, [&](auto t) {
-        hipLaunchKernelGGL((attn_prompt_kernel<decltype(t)>), dim3(p->n_q, p->heads), dim3(AT_NT), 0, c->stream, a);
+        using T = decltype(t);
+        if (p->dim <= 64) p->dim == 64 ? launch_prompt<T, 64, true>(c, a) : launch_prompt<T, 64, false>(c, a);
+        else if (p->dim <= 128) p->dim == 128 ? launch_prompt<T, 128, true>(c, a) : launch_prompt<T, 128, false>(c, a);
+        else p->dim == 256 ? launch_prompt<T, 256, true>(c, a) : launch_prompt<T, 256, false>(c, a);
     });
     return finish(c);
 }

@@ -271,7 +271,8 @@ typedef struct {
     float scale;
     uint32_t window;                /* 0: none */
 } okf_attn;
-/* Pointers are 16-byte aligned and strides whole multiples of 16 bytes. */
+/* Pointers are 16-byte aligned, strides whole multiples of 16 bytes, the row
+ * strides of k and v at most 2^23 values. */
 int okf_attn_prompt(okf_ctx *ctx, const okf_attn *a);
 
 /* A paged KV cache: a page holds OKF_KV_BLOCK tokens of every head, as int8
