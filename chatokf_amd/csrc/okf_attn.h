@@ -168,7 +168,8 @@ __global__ __launch_bounds__(AT_NT, AtType<T>::NP == 1 && DP <= 128 ? 2 : 1) voi
     }
     auto issue = [&](int j, int buf) {
         if constexpr (NP == 1) {
-            // rows past the sequence's end lie past the buffer's
+            // rows past the sequence's end lie past the buffer's (whole offsets in the lanes: the
+            // range check may leave the scalar one out)
             const uint32_t rows = (uint32_t)min(nk - j, BN);
             auto rk_ = __builtin_amdgcn_make_buffer_rsrc((void *)(kp + (uint64_t)j * a.ks), 0,
                                                          (rows - 1) * (uint32_t)(a.ks * 2) + D * 2, 0x00027000);
@@ -178,12 +179,12 @@ __global__ __launch_bounds__(AT_NT, AtType<T>::NP == 1 && DP <= 128 ? 2 : 1) voi
             uint8_t *to = at_mem + buf * 2 * PB + wave * 1024;
 #pragma unroll
             for (int p = 0; p < PIECES; p++)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rk_, (lds_t *)(to + p * 4096), 16, koff[p & 1],
-                                                         p * 4 * RPP * (uint32_t)(a.ks * 2), 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rk_, (lds_t *)(to + p * 4096), 16,
+                                                         koff[p & 1] + p * 4 * RPP * (uint32_t)(a.ks * 2), 0, 0, 0);
 #pragma unroll
             for (int p = 0; p < PIECES; p++)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rv_, (lds_t *)(to + PB + p * 4096), 16, voff,
-                                                         p * 4 * RPP * (uint32_t)(a.vs * 2), 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rv_, (lds_t *)(to + PB + p * 4096), 16,
+                                                         voff + p * 4 * RPP * (uint32_t)(a.vs * 2), 0, 0, 0);
         } else {
 #pragma unroll
             for (int i = 0; i < XV; i++) {
