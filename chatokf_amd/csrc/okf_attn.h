@@ -320,7 +320,8 @@ __global__ __launch_bounds__(AT_NT, AtType<T>::NP == 1 && DP <= 128 ? 2 : 1) voi
             for (int d = 0; d < DT; d++) o[d] *= f;
             m = nm;
         }
-        const float mc = m == -__builtin_inff() ? 0.0f : m * c;
+        // (f16: weights up to 2^8 2^7, so that those 2^-30 of the largest are still normal or nearly so)
+        const float mc = (m == -__builtin_inff() ? 0.0f : m * c) - (__is_same(E, _Float16) ? 7.0f : 0.0f);
         u32x4v p[NP][2 * TT];
 #pragma unroll
         for (int t = 0; t < TT; t++)

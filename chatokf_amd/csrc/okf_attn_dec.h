@@ -7,8 +7,10 @@
 // v_mfma_i32_16x16x64_i8 against the codes as they lie in memory.  Their sums
 // are exact in 32 bits ((Q1 code << 8) + Q0 code too), so a score's roundings
 // are Q's (2^-24 of the row's largest) and a few in fp32.  The softmax weights p
-// <= 1 (of the running maximum) become P = rint(p (2^23 - 2^15 - 2^7 - 1)) the
-// same way for the product with the value codes.  No code is ever unpacked.
+// <= 1 of the page's largest score become P = rint(p (2^23 - 2^15 - 2^7 - 1)) the
+// same way for the product with the value codes (against the running maximum, one
+// token that takes nearly all would leave the others' integers no digits).  No code
+// is ever unpacked.
 //
 // Layout.  A wavefront takes one page (64 tokens) at a time and 16 NR query rows
 // (row = query token * group + query head of the group).  Scores: A = 16 tokens
@@ -253,14 +255,17 @@ __global__ __launch_bounds__(DEC_NT, KS * NR <= 2 ? 2 : 1) void attn_dec_kernel(
                     for (int d = 0; d < 4 * KS; d++) o[n][d] *= f;
                 }
                 m[n] = nm;
+                // weights of the page's own largest score, which g brings to the running one
+                const float own = x == -__builtin_inff() ? 0.0f : x, g = __builtin_amdgcn_exp2f(x - ref);
+                float lp = 0;
                 int32x4 pd[3];
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
                     uint32_t y[4];
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const float p = __builtin_amdgcn_exp2f(s[n][4 * t + i] - ref);
-                        l[n] += p;
+                        const float p = __builtin_amdgcn_exp2f(s[n][4 * t + i] - own);
+                        lp += p;
                         // (2^23 + P: P's rounding is the addition's, its digits the low three bytes)
                         y[i] = __float_as_uint(fmaf(p, DEC_P, 8388608.0f)) + 0x808080u;
                     }
@@ -269,7 +274,8 @@ __global__ __launch_bounds__(DEC_NT, KS * NR <= 2 ? 2 : 1) void attn_dec_kernel(
                     pd[0][t] = d0, pd[1][t] = d1, pd[2][t] = d2;
                 }
                 // (a row that sees nothing of the page takes nothing from it, a NaN scale neither)
-                const float f = j0 < q.hi[n] && j0 + KV_B > q.lo[n] ? vs : 0.0f;
+                const float f = j0 < q.hi[n] && j0 + KV_B > q.lo[n] ? vs * g : 0.0f;
+                l[n] = fmaf(lp, g, l[n]);
 #pragma unroll
                 for (int d = 0; d < 4 * KS; d++)
                     if (16u * d < D) {

@@ -254,6 +254,21 @@ def test_prompt_extremes(enc, t):
 
 
 @gpu
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_prompt_one_key_takes_nearly_all(enc, t):
+    """The other 5999 keys, 2^-20.5 of the first each, keep their part of the output (whose
+    value at the first key is 0): a weight's and the output's half step, and the sums' u."""
+    n, D = 6000, 64
+    q, k, v = torch.zeros(1, 1, D), torch.zeros(n, 1, D), torch.ones(n, 1, D)
+    q[..., 0], k[0, 0, 0], v[0] = 4.0, 8.0, 0.0
+    scale = 20.5 * np.log(2) / 32
+    got = run_prompt(enc, *(x.to(TYPES[t]).cuda() for x in (q, k, v)), [0, 1], [0, n], t, 0, scale, 1, 1, D)
+    w = (n - 1) * 2.0 ** -20.5
+    ref = w / (1 + w)
+    assert np.abs(got / ref - 1).max() <= (2 * n + 100) * U + (0 if t == "f32" else torch.finfo(TYPES[t]).eps)
+
+
+@gpu
 def test_prompt_bad_starts(enc):
     """Starts that leave the rows or decrease are clamped: nothing outside is read or written."""
     n, D = 70, 64
@@ -529,6 +544,25 @@ def test_decode_extreme_queries(enc):
         bound = tol(q[0, 0, h:h + 1] * 8, np.full((1, 64), 5.2), np.full(1, 5.2), 0.1, 200, 64)
         assert np.abs(got[0, 0, h] - ref[0, 0, h]).max() <= bound, h
     assert np.isnan(got[0, 0, 6]).all() and not np.isfinite(got[0, 0, 7]).any()
+
+
+@gpu
+def test_decode_one_token_takes_nearly_all(enc):
+    """The other tokens, 2^-27.5 of the first each, keep their part of the output (whose values
+    in the first page are 0): the sums' u, 2^-23 of each page's weights, a score's few u times 19."""
+    d = Dev([6400], 1, 64, 14)
+    d.c.k[:], d.c.v[:], d.c.ks[:], d.c.vs[:] = 0, 100, 1, 0.01
+    first = d.table[0, 0]
+    d.c.k[first, 0, 0, 0], d.c.v[first] = 127, 0
+    d.push()
+    q = np.zeros((1, 1, 1, 64), np.float32)
+    q[..., 0] = 1
+    o = torch.empty(q.shape, device="cuda")
+    enc.attn_decode(d.cache, d.seqs, dev(q), o, 1, 1, 27.5 * np.log(2) / 127)
+    enc.sync()
+    w = 2.0 ** -27.5
+    ref = 6336 * w / (1 + 6399 * w) * 100 * np.float64(np.float32(0.01))
+    assert np.abs(host(o) / ref - 1).max() <= (2 * 6400 + 200) * U
 
 
 @gpu
