@@ -1,8 +1,9 @@
 // okf_attn.hip -- the C ABI of attention and the KV cache (include/okf_quant.h)
 // over okf_attn.h, okf_attn_dec.h and okf_kv.h.
 #include "okf_impl.h"
-#include "okf_attn.h"
+#include "okf_attn_run.h"
 #include "okf_attn_dec.h"
+#include "okf_kv.h"
 
 namespace {
 
@@ -62,13 +63,6 @@ int check_rows(const okf_kv_cache *c, const okf_kv_seqs *s, const void *k, const
     if (items > 0x7FFFFFFFull) return OKF_E_SHAPE;
     grid = dim3((uint32_t)items, c->heads, 2);
     return OKF_OK;
-}
-
-template <class T, int DP, bool FULL>
-void launch_prompt(okf_ctx *c, const AttnArgs &a) {
-    static std::atomic<uint64_t> attr{0};
-    set_lds_attr(c, (const void *)attn_prompt_kernel<T, DP, FULL>, attr);
-    hipLaunchKernelGGL((attn_prompt_kernel<T, DP, FULL>), dim3(a.tiles * a.heads), dim3(AT_NT), (at_lds<T, DP>()), c->stream, a);
 }
 
 // The splits of okf_attn_decode: how many page ranges each sequence and kv head
@@ -151,17 +145,10 @@ int okf_attn_prompt(okf_ctx *c, const okf_attn *p) {
         return OKF_E_SHAPE;
     int st = begin(c);
     if (st) return st;
-    // (sequences' tiles: at most n_q / 128 and one each; never more than the rows)
-    const uint64_t tiles = std::min<uint64_t>((uint64_t)p->n_q / AT_BM + p->seqs, p->n_q);
-    if (tiles * p->heads > 0x7FFFFFFFull) return OKF_E_SHAPE;
-    a.tiles = (uint32_t)tiles;
-    with_type(p->type, [&](auto t) {
-        using T = decltype(t);
-        if (p->dim <= 64) p->dim == 64 ? launch_prompt<T, 64, true>(c, a) : launch_prompt<T, 64, false>(c, a);
-        else if (p->dim <= 128) p->dim == 128 ? launch_prompt<T, 128, true>(c, a) : launch_prompt<T, 128, false>(c, a);
-        else p->dim == 256 ? launch_prompt<T, 256, true>(c, a) : launch_prompt<T, 256, false>(c, a);
-    });
-    return finish(c);
+    if (p->type == F32) st = launch_prompt<float>(c, a);
+    else if (p->type == F16) st = launch_prompt<_Float16>(c, a);
+    else st = launch_prompt<__bf16>(c, a);
+    return st ? st : finish(c);
 }
 
 int okf_attn_decode(okf_ctx *c, const okf_kv_cache *cache, const okf_kv_seqs *seqs, const float *q, float *o,

@@ -21,8 +21,8 @@
 // the value rows: no exchange between lanes, and no LDS, until the wavefronts
 // of a workgroup join their results at the end.
 #pragma once
-#include "okf_attn.h"
 #include "okf_ffn_mfma.h"
+#include "okf_kv_seqs.h"
 
 namespace okf {
 

@@ -8,66 +8,14 @@
 // kernel's matrix instruction takes them (kv_slot), so that it loads both
 // without a transpose.
 #pragma once
-#include "okf_common.h"
+#include "okf_kv_seqs.h"
 
 namespace okf {
-
-constexpr uint32_t KV_B = 64;  // tokens a page
 
 // where token t of a page stands in a value row, and the token at byte b of
 // 16-byte group g
 __host__ __device__ constexpr uint32_t kv_slot(uint32_t t) { return t % 16 / 4 * 16 + t / 16 * 4 + t % 4; }
 __host__ __device__ constexpr uint32_t kv_token(uint32_t g, uint32_t b) { return b / 4 * 16 + g * 4 + b % 4; }
-
-struct KvCache {
-    int8_t *k, *v;
-    float *ks, *vs;
-    uint32_t pages, heads, dim;
-};
-
-struct KvSeqs {
-    const int32_t *pages;
-    int32_t *len;
-    uint32_t count, stride;
-};
-
-__device__ __forceinline__ float to_f32(float x) { return x; }
-__device__ __forceinline__ float to_f32(_Float16 x) { return (float)x; }
-__device__ __forceinline__ float to_f32(__bf16 x) { return (float)x; }
-
-// The sequence that item idx belongs to when sequence s has items(s) of them,
-// and the item's place in it; seq = count past the last.  Every lane of the
-// wavefront calls this with the same idx and gets the same answer.
-struct SeqItem {
-    uint32_t seq, at;
-};
-template <class F>
-__device__ __forceinline__ SeqItem kv_find(uint32_t idx, uint32_t count, F items) {
-    const uint32_t lane = threadIdx.x & 63;
-    uint64_t before = 0;
-    for (uint32_t b = 0; b < count; b += 64) {
-        const uint32_t n = b + lane < count ? items(b + lane) : 0;
-        uint64_t sum = n;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint64_t v = __shfl_up(sum, o);
-            if (lane >= (uint32_t)o) sum += v;
-        }
-        const uint64_t here = __ballot(before + sum > idx);
-        if (here) {
-            const int l = __ffsll((unsigned long long)here) - 1;
-            return {b + l, idx - (uint32_t)(before + __shfl(sum - n, l))};
-        }
-        before += __shfl(sum, 63);
-    }
-    return {count, 0};
-}
-
-// The rows [a, b) that packed starts give a sequence, inside [0, n].
-__device__ __forceinline__ uint2 kv_rows(const int32_t *start, uint32_t s, uint32_t n) {
-    const uint32_t a = (uint32_t)min(max(start[s], 0), (int)n);
-    return {a, (uint32_t)min(max(start[s + 1], (int)a), (int)n)};
-}
 
 // The page blocks that a sequence's last n rows touch: positions old .. len - 1.
 struct KvSpan {

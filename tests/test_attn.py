@@ -182,6 +182,43 @@ def test_prompt(enc, t, H, KV, D, qlens, klens, window):
 
 @gpu
 @pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("H,KV,D,qlens,klens,window", [
+    (2, 1, 128, [70], [1500], 0),                               # few rows, many keys: the keys over four groups
+    (3, 1, 64, [33, 100], [900, 1200], 0),
+    (2, 2, 80, [129], [1000], 900),
+    (2, 1, 96, [65], [1024], 0),
+    (2, 1, 256, [100], [800], 0),
+    (48, 4, 64, [300, 1, 513], None, 0),                        # many rows: 128 a workgroup
+    (48, 4, 128, [300, 1, 513], None, 77),
+    (32, 8, 96, [700, 400], [700, 900], 0),
+    (130, 2, 256, [290], None, 0),
+    (16, 2, 64, [i * 7 % 13 for i in range(80)], None, 0),      # more sequences than a wavefront has lanes
+    (2, 2, 64, [5, 0, 300, 64, 1, 129], [5, 7, 900, 1000, 1, 500], 0),  # tiles of the most keys first
+])
+def test_prompt_workgroups(enc, t, H, KV, D, qlens, klens, window):
+    """The shapes of workgroups that the sizes choose, and the orders of their tiles."""
+    test_prompt(enc, t, H, KV, D, qlens, klens, window)
+
+
+@gpu
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("H,n,before", [(2, 60, 1000), (40, 900, 0), (2, 100, 50)])
+def test_prompt_unseen_by_workgroups(enc, t, H, n, before):
+    """A NaN value and an infinite key half way: rows before them are as ever, all others show it."""
+    rng = np.random.default_rng(16)
+    D, m = 64, n + before
+    at = before + n // 2
+    q, k, v = (rng.standard_normal((r, h, D)).astype(np.float32) for r, h in ((n, H), (m, 1), (m, 1)))
+    q_, k_, v_ = (dev(x, TYPES[t]) for x in (q, k, v))
+    ref = ao.prompt(host(q_), host(k_), host(v_), [0, n], [0, m], 0, 0.1)
+    v_[at, 0, 9], k_[at + 1, 0, 3] = float("nan"), float("inf")
+    got = run_prompt(enc, q_, k_, v_, [0, n], [0, m], t, 0, 0.1, H, 1, D)
+    assert np.abs(got[:n // 2] - ref[:n // 2]).max() <= tol(host(dev(q, TYPES[t])), k, v, 0.1, m, D, t)
+    assert not np.isfinite(got[n // 2:, :, 9]).any()
+
+
+@gpu
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
 def test_prompt_strides(enc, t):
     """Rows of a fused projection, and a head-major layout; the gaps are left alone."""
     rng = np.random.default_rng(5)
