@@ -159,14 +159,9 @@ __device__ __forceinline__ SeqItem at_tile(const AttnArgs &a, uint32_t idx) {
     }
     auto count = [&](uint32_t level) {  // tiles of this level and above
         uint32_t v = level < before + n ? min(before + n - level, n) : 0;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
-        return (uint32_t)__builtin_amdgcn_readfirstlane(v);
+        return (uint32_t)__builtin_amdgcn_readlane(lanes_sum(v), 63);
     };
-    uint32_t lo = 0, hi = before + n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) hi = max(hi, (uint32_t)__shfl_xor(hi, o));
-    hi = __builtin_amdgcn_readfirstlane(hi);  // count(lo) > idx >= count(hi)
+    uint32_t lo = 0, hi = lanes_max(before + n);  // count(lo) > idx >= count(hi)
     if (count(0) <= idx) return {a.seqs, 0};
     uint32_t above = 0;
     while (hi - lo > 1) {

@@ -22,6 +22,17 @@ void with_type(int32_t t, Fn f) {
     else f(__bf16{});
 }
 
+// Runs f with the 64s of dimensions that hold dim, as a constant.
+template <class Fn>
+void with_dims(uint32_t dim, Fn f) {
+    switch ((dim + 63) / 64) {
+    case 1: f(std::integral_constant<int, 1>{}); break;
+    case 2: f(std::integral_constant<int, 2>{}); break;
+    case 3: f(std::integral_constant<int, 3>{}); break;
+    default: f(std::integral_constant<int, 4>{}); break;
+    }
+}
+
 bool good_dim(uint32_t d) { return d >= 16 && d <= 256 && d % 16 == 0; }
 
 int check_cache(const okf_kv_cache *c) {
@@ -168,12 +179,7 @@ int okf_attn_decode(okf_ctx *c, const okf_kv_cache *cache, const okf_kv_seqs *se
               nullptr, nullptr};
     if ((st = plan_decode(c, a))) return st;
     if (a.ml) note_capture(c, false, true, false);
-    switch ((cache->dim + 63) / 64) {
-    case 1: launch_decode<1>(c, a, rows > 16); break;
-    case 2: launch_decode<2>(c, a, rows > 16); break;
-    case 3: launch_decode<3>(c, a, rows > 16); break;
-    default: launch_decode<4>(c, a, rows > 16); break;
-    }
+    with_dims(cache->dim, [&](auto ks) { launch_decode<decltype(ks)::value>(c, a, rows > 16); });
     return finish(c);
 }
 
@@ -186,8 +192,10 @@ int okf_kv_append(okf_ctx *c, const okf_kv_cache *cache, const okf_kv_seqs *seqs
     if ((st = begin(c))) return st;
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        hipLaunchKernelGGL((kv_append_kernel<T>), grid, dim3(KV_NT), 0, c->stream, cache_of(cache), seqs_of(seqs),
-                           (const T *)k, (const T *)v, start, n, k_stride, v_stride);
+        with_dims(cache->dim, [&](auto nd) {
+            hipLaunchKernelGGL((kv_append_kernel<T, decltype(nd)::value>), grid, dim3(KV_NT), 0, c->stream, cache_of(cache),
+                               seqs_of(seqs), (const T *)k, (const T *)v, start, n, k_stride, v_stride);
+        });
     });
     return finish(c);
 }
@@ -201,8 +209,10 @@ int okf_kv_read(okf_ctx *c, const okf_kv_cache *cache, const okf_kv_seqs *seqs, 
     if ((st = begin(c))) return st;
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        hipLaunchKernelGGL((kv_read_kernel<T>), grid, dim3(KV_NT), 0, c->stream, cache_of(cache), seqs_of(seqs),
-                           (T *)k, (T *)v, start, n, k_stride, v_stride);
+        with_dims(cache->dim, [&](auto nd) {
+            hipLaunchKernelGGL((kv_read_kernel<T, decltype(nd)::value>), grid, dim3(KV_NT), 0, c->stream, cache_of(cache),
+                               seqs_of(seqs), (T *)k, (T *)v, start, n, k_stride, v_stride);
+        });
     });
     return finish(c);
 }
@@ -230,8 +240,11 @@ int okf_kv_evict(okf_ctx *c, const okf_kv_cache *src, const okf_kv_seqs *from, c
     if ((st = begin(c))) return st;
     hipLaunchKernelGGL(kv_select_kernel, dim3((uint32_t)rows), dim3(EV_NT), 0, c->stream, seqs_of(from), to->len,
                        src->heads, keep, sink, recent, w_in, w_in_stride, w_out, w_out_stride, kept);
-    hipLaunchKernelGGL(kv_gather_kernel, dim3((keep + KV_B - 1) / KV_B, group * src->heads, groups), dim3(KV_NT), 0,
-                       c->stream, cache_of(src), seqs_of(from), cache_of(dst), seqs_of(to), keep, kept);
+    const dim3 grid((keep + KV_B - 1) / KV_B, group * src->heads, groups);
+    with_dims(src->dim, [&](auto nd) {
+        hipLaunchKernelGGL(kv_gather_kernel<decltype(nd)::value>, grid, dim3(KV_NT), 0, c->stream, cache_of(src), seqs_of(from),
+                           cache_of(dst), seqs_of(to), keep, (const int32_t *)kept);
+    });
     return finish(c);
 }
 

@@ -285,7 +285,7 @@ int okf_attn_prompt(okf_ctx *ctx, const okf_attn *a);
 #define OKF_KV_BLOCK 64
 typedef struct {
     int8_t *k, *v;
-    float *k_scale, *v_scale;       /* [page][head] */
+    float *k_scale, *v_scale;       /* [page][head], never negative */
     uint32_t pages, heads, dim;     /* heads: the kv heads */
 } okf_kv_cache;
 
@@ -313,8 +313,8 @@ int okf_kv_append(okf_ctx *ctx, const okf_kv_cache *cache, const okf_kv_seqs *se
                   int32_t type, const int32_t *start, uint32_t n, uint64_t k_stride, uint64_t v_stride);
 
 /* Reads values back: the last start[s + 1] - start[s] tokens of sequence s to
- * the rows from start[s] of k and v (either may be NULL), code * scale rounded
- * once to `type`: what okf_attn_prompt takes for a chunk behind a cached
+ * the rows from start[s] of k and v (either may be NULL), code * scale in fp32,
+ * then rounded to `type`: what okf_attn_prompt takes for a chunk behind a cached
  * prefix.  Rows past the sequence's beginning are 0. */
 int okf_kv_read(okf_ctx *ctx, const okf_kv_cache *cache, const okf_kv_seqs *seqs, void *k, void *v, int32_t type,
                 const int32_t *start, uint32_t n, uint64_t k_stride, uint64_t v_stride);
