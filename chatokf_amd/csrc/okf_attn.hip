@@ -78,8 +78,7 @@ int check_rows(const okf_kv_cache *c, const okf_kv_seqs *s, const void *k, const
 
 // The splits of okf_attn_decode: how many page ranges each sequence and kv head
 // is cut into, so that the workgroups fill the CUs (as many at a time on each as the
-// kernel's registers leave room for: two for 16 rows of up to 128 dimensions or 32 of
-// up to 64, one past that), but no range of less than a page for each of a
+// kernel's registers leave room for: two for up to 128 dimensions, one past that), but no range of less than a page for each of a
 // workgroup's wavefronts; batches of ragged sequences get twice that, so that the
 // short ones' workgroups make room for the long ones'.  The partial results go to
 // the context's buffer; where it may not grow, as many splits as it holds.
@@ -87,9 +86,9 @@ int plan_decode(okf_ctx *c, DecArgs &a) {
     const uint64_t rows = (uint64_t)a.tokens * (a.heads / a.c.heads), rpb = rows > 16 ? 32 : 16;
     a.rb = (uint32_t)((rows + rpb - 1) / rpb);
     const uint64_t base = (uint64_t)a.s.count * a.c.heads * a.rb;
-    uint64_t want = (uint64_t)c->cus * (a.c.dim * rpb <= 2048 ? 2 : 1) * (a.s.count > 1 ? 2 : 1);
+    uint64_t want = (uint64_t)c->cus * (a.c.dim <= 128 ? 2 : 1) * (a.s.count > 1 ? 2 : 1);
     const uint64_t span = a.window ? std::min<uint64_t>(((uint64_t)a.window + a.tokens) / KV_B + 2, a.s.stride) : a.s.stride;
-    uint64_t splits = std::max<uint64_t>(1, std::min((want + base - 1) / base, (span + DEC_W - 1) / DEC_W));
+    uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>({(want + base - 1) / base, (span + DEC_W - 1) / DEC_W, DEC_SPLITS}));
     auto bytes = [&](uint64_t n) {  // m and l, then partial outputs
         return base * n * rpb * 2 * sizeof(float) + (n > 1 ? base * n * rpb * a.c.dim * sizeof(float) : 0);
     };
@@ -113,7 +112,7 @@ void launch_decode_n(okf_ctx *c, const DecArgs &a) {
     static std::atomic<uint64_t> attr{0};
     set_lds_attr(c, (const void *)attn_dec_kernel<KS, NR>, attr);
     const uint32_t sh = a.s.count * a.c.heads;
-    const size_t lds = (size_t)DEC_W * 16 * NR * (a.c.dim + 4 + 2) * sizeof(float);
+    const size_t lds = (size_t)DEC_W * 16 * (a.c.dim + 4 + 2) * sizeof(float);
     hipLaunchKernelGGL((attn_dec_kernel<KS, NR>), dim3((sh * a.splits + 7) / 8 * 8 * a.rb), dim3(DEC_NT), lds, c->stream, a);
     if (a.splits > 1)
         hipLaunchKernelGGL(attn_dec_join_kernel, dim3(sh * a.tokens * (a.heads / a.c.heads)), dim3(DEC_NT), 0, c->stream, a,

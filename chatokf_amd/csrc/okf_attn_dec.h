@@ -12,14 +12,21 @@
 // token that takes nearly all would leave the others' integers no digits).  No code
 // is ever unpacked.
 //
-// Layout.  A wavefront takes one page (64 tokens) at a time and 16 NR query rows
-// (row = query token * group + query head of the group).  Scores: A = 16 tokens
+// Layout.  A wavefront takes one page (64 tokens) at a time and 16 query rows
+// (row = query token * group + query head of the group); where there are more, two
+// wavefronts of a workgroup take a page each with 16 rows of their own.  Scores: A = 16 tokens
 // x 64 dimensions of K, B = a digit plane of the queries; a lane then holds,
 // for the query row lane % 16, tokens 16 t + 4 (lane / 16) + i.  Values: A = 16
 // dimensions x the page's 64 tokens, B = a digit plane of P, whose 16 bytes a lane
 // are just the tokens whose scores it holds, in the order that kv_slot gives
 // the value rows: no exchange between lanes, and no LDS, until the wavefronts
 // of a workgroup join their results at the end.
+//
+// Bound by the cache's bytes for batches (32 sequences of up to 8192 tokens, 8 kv heads of
+// 128: 56 us, 5.2 TB/s, as fast as a copy), by the chain of loads (length, page, scale, keys)
+// and the second launch for one short sequence (1999 tokens 7.3 + 3.6 us), by latency and the
+// vector units for wide heads (100003 tokens x 4 x 256, 20 rows each: 58 us, 3.5 TB/s: one
+// wavefront a SIMD; two, with the values in the keys' registers, spill: 100 us).
 #pragma once
 #include "okf_ffn_mfma.h"
 #include "okf_kv_seqs.h"
@@ -123,14 +130,17 @@ struct DecQuery {
 
 // The keys of a page as the A operand: tile t, dimensions 64 k + 16 (lane / 16) ..
 template <int KS>
-__device__ __forceinline__ void dec_load_k(int32x4 (&kk)[4][KS], const int8_t *page, uint32_t D) {
+__device__ __forceinline__ void dec_load_tile(int32x4 (&kk)[KS], int t, const int8_t *page, uint32_t D) {
     const uint32_t lane = threadIdx.x & 63;
-    const int8_t *p = page + (lane & 15) * D;
+    const int8_t *p = page + ((lane & 15) + 16 * t) * D;
 #pragma unroll
-    for (int t = 0; t < 4; t++)
+    for (int k = 0; k < KS; k++)  // (past the end: bytes of the row that meet zero digits)
+        kk[k] = *(const int32x4 *)(p + min(64 * k + 16 * (lane >> 4), D - 16));
+}
+template <int KS>
+__device__ __forceinline__ void dec_load_k(int32x4 (&kk)[4][KS], const int8_t *page, uint32_t D) {
 #pragma unroll
-        for (int k = 0; k < KS; k++)  // (past the end: bytes of the row that meet zero digits)
-            kk[t][k] = *(const int32x4 *)(p + 16 * t * D + min(64 * k + 16 * (lane >> 4), D - 16));
+    for (int t = 0; t < 4; t++) dec_load_tile<KS>(kk[t], t, page, D);
 }
 
 // Scores of a page in units of log2, masked where the page is not wholly visible.
@@ -187,28 +197,41 @@ __device__ __forceinline__ DecAt dec_at(const DecArgs &a, uint32_t id) {
     return {sh / a.c.heads, sh % a.c.heads, i % a.splits, rb, sh < a.s.count * a.c.heads};
 }
 
-template <int KS, int NR>
-__global__ __launch_bounds__(DEC_NT, KS * NR <= 2 ? 2 : 1) void attn_dec_kernel(DecArgs a) {
-    extern __shared__ __align__(16) float dec_lds[];  // [wave][16 NR][dim + 4], then m and l [wave][16 NR]
+// Visible pages of a block of rows, as its first and last row see them.
+__device__ __forceinline__ uint2 dec_block_pages(const DecArgs &a, uint32_t s, uint32_t r0, uint32_t r1) {
+    const uint32_t G = a.heads / a.c.heads;
+    const int64_t len = max(a.s.len[s], 0);
+    const uint32_t cap = (uint32_t)min(len, (int64_t)a.s.stride * KV_B);
+    const int64_t e0 = max(len - a.tokens + r0 / G + 1, (int64_t)0), e1 = max(len - a.tokens + r1 / G + 1, (int64_t)0);
+    return dec_pages(a.window && e0 > a.window ? (uint32_t)(e0 - a.window) : 0, (uint32_t)min(e1, (int64_t)cap));
+}
+
+// RB: the blocks of 16 rows that a workgroup's wavefronts are dealt to (1 or 2); the
+// wavefronts of a block take its pages in turn.  (Both blocks in each wavefront, which
+// reads every page once, takes 490 registers and the same time, 59 us for the longest
+// case above.)
+template <int KS, int RB>
+__global__ __launch_bounds__(DEC_NT, KS <= 2 ? 2 : 1) void attn_dec_kernel(DecArgs a) {
+    extern __shared__ __align__(16) float dec_lds[];  // [wave][16][dim + 4], then m and l [wave][16]
     float *const lds = dec_lds;
+    constexpr uint32_t PW = DEC_W / RB;
     const DecAt at = dec_at(a, blockIdx.x);
     if (!at.ok) return;
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, D = a.c.dim, g4 = lane >> 4;
-    DecQuery<KS, NR> q;
-    q.load(a, at.s, at.kh, at.rb);
-    const uint2 pg = dec_pages(q.lo_min, q.hi_max);
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), D = a.c.dim, g4 = lane >> 4;
+    const uint32_t G = a.heads / a.c.heads, rows = a.tokens * G, r0 = at.rb * 16 * RB;
+    DecQuery<KS, 1> q;
+    q.load(a, at.s, at.kh, at.rb * RB + wave % RB);
+    const uint2 pg = dec_block_pages(a, at.s, r0, min(r0 + 16 * RB, rows) - 1);
     const uint32_t chunk = dec_chunk(pg, a.splits);
     const uint32_t p0 = pg.x + at.split * chunk, p1 = min(p0 + chunk, pg.y);
     if (a.splits > 1 && p0 >= p1) return;  // (the joining kernel knows)
-    floatx4 o[NR][4 * KS] = {};
-    float m[NR], l[NR];
-#pragma unroll
-    for (int n = 0; n < NR; n++) m[n] = -__builtin_inff(), l[n] = 0;
+    floatx4 o[4 * KS] = {};
+    float m = -__builtin_inff(), l = 0;
     const int32_t *pages = a.s.pages + (uint64_t)at.s * a.s.stride;
     const uint64_t pbytes = (uint64_t)KV_B * D;
-    for (uint32_t b = p0 + wave; b < p1; b += 64 * DEC_W) {
+    for (uint32_t b = p0 + wave / RB; b < p1; b += 64 * PW) {
         // page ids and scales of this wavefront's next 64 pages, one a lane
-        const uint32_t mine = b + lane * DEC_W;
+        const uint32_t mine = b + lane * PW;
         const int32_t id = mine < p1 ? pages[mine] : -1;
         const bool have = (uint32_t)id < a.c.pages;
         const uint64_t ph = have ? (uint64_t)id * a.c.heads + at.kh : 0;
@@ -224,7 +247,7 @@ __global__ __launch_bounds__(DEC_NT, KS * NR <= 2 ? 2 : 1) void attn_dec_kernel(
         uint64_t off = base(at_lane);
         dec_load_k<KS>(kk, a.c.k + off, D);
         while (todo) {
-            const uint32_t j0 = (b + at_lane * DEC_W) * KV_B;
+            const uint32_t j0 = (b + at_lane * PW) * KV_B;
             const float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lks), at_lane));
             const float vs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lvs), at_lane));
             int32x4 vv[4 * KS];
@@ -232,159 +255,175 @@ __global__ __launch_bounds__(DEC_NT, KS * NR <= 2 ? 2 : 1) void attn_dec_kernel(
 #pragma unroll
             for (int d = 0; d < 4 * KS; d++)
                 if (16u * d < D) vv[d] = *(const int32x4 *)(vp + d * 1024);
-            float s[NR][16];
-            dec_scores<KS, NR>(s, kk, q, ks, j0);
+            float s[1][16];
+            dec_scores<KS, 1>(s, kk, q, ks, j0);
             todo &= todo - 1;
             if (todo) {
                 at_lane = __ffsll((unsigned long long)todo) - 1;
                 off = base(at_lane);
                 dec_load_k<KS>(kk, a.c.k + off, D);
             }
+            float x = s[0][0];
 #pragma unroll
-            for (int n = 0; n < NR; n++) {
-                float x = s[n][0];
+            for (int i = 1; i < 16; i++) x = fmaxf(x, s[0][i]);
+            x = fmaxf(x, __shfl_xor(x, 16));
+            x = fmaxf(x, __shfl_xor(x, 32));
+            const float nm = fmaxf(m, x), ref = nm == -__builtin_inff() ? 0.0f : nm;
+            if (__ballot(nm > m)) {
+                const float f = __builtin_amdgcn_exp2f(m - ref);
+                l *= f;
 #pragma unroll
-                for (int i = 1; i < 16; i++) x = fmaxf(x, s[n][i]);
-                x = fmaxf(x, __shfl_xor(x, 16));
-                x = fmaxf(x, __shfl_xor(x, 32));
-                const float nm = fmaxf(m[n], x), ref = nm == -__builtin_inff() ? 0.0f : nm;
-                if (__ballot(nm > m[n])) {
-                    const float f = __builtin_amdgcn_exp2f(m[n] - ref);
-                    l[n] *= f;
-#pragma unroll
-                    for (int d = 0; d < 4 * KS; d++) o[n][d] *= f;
-                }
-                m[n] = nm;
-                // weights of the page's own largest score, which g brings to the running one
-                const float own = x == -__builtin_inff() ? 0.0f : x, g = __builtin_amdgcn_exp2f(x - ref);
-                float lp = 0;
-                int32x4 pd[3];
-#pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    uint32_t y[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float p = __builtin_amdgcn_exp2f(s[n][4 * t + i] - own);
-                        lp += p;
-                        // (2^23 + P: P's rounding is the addition's, its digits the low three bytes)
-                        y[i] = __float_as_uint(fmaf(p, DEC_P, 8388608.0f)) + 0x808080u;
-                    }
-                    int d0, d1, d2;
-                    dec_digits(y[0], y[1], y[2], y[3], d0, d1, d2);
-                    pd[0][t] = d0, pd[1][t] = d1, pd[2][t] = d2;
-                }
-                // (a row that sees nothing of the page takes nothing from it, a NaN scale neither)
-                const float f = j0 < q.hi[n] && j0 + KV_B > q.lo[n] ? vs * g : 0.0f;
-                l[n] = fmaf(lp, g, l[n]);
-#pragma unroll
-                for (int d = 0; d < 4 * KS; d++)
-                    if (16u * d < D) {
-                        const int32x4 z = {0, 0, 0, 0};
-                        const int32x4 c0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(vv[d], pd[0], z, 0, 0, 0);
-                        const int32x4 c1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(vv[d], pd[1], z, 0, 0, 0);
-                        const int32x4 c2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(vv[d], pd[2], z, 0, 0, 0);
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            o[n][d][i] += fmaf((float)c2[i], 65536.0f, (float)((c1[i] << 8) + c0[i])) * f;
-                    }
+                for (int d = 0; d < 4 * KS; d++) o[d] *= f;
             }
+            m = nm;
+            // weights of the page's own largest score, which g brings to the running one
+            const float own = x == -__builtin_inff() ? 0.0f : x, g = __builtin_amdgcn_exp2f(x - ref);
+            float lp = 0;
+            int32x4 pd[3];
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                uint32_t y[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float p = __builtin_amdgcn_exp2f(s[0][4 * t + i] - own);
+                    lp += p;
+                    // (2^23 + P: P's rounding is the addition's, its digits the low three bytes)
+                    y[i] = __float_as_uint(fmaf(p, DEC_P, 8388608.0f)) + 0x808080u;
+                }
+                int d0, d1, d2;
+                dec_digits(y[0], y[1], y[2], y[3], d0, d1, d2);
+                pd[0][t] = d0, pd[1][t] = d1, pd[2][t] = d2;
+            }
+            // (a row that sees nothing of the page takes nothing from it, a NaN scale neither)
+            const float f = j0 < q.hi[0] && j0 + KV_B > q.lo[0] ? vs * g : 0.0f;
+            l = fmaf(lp, g, l);
+#pragma unroll
+            for (int d = 0; d < 4 * KS; d++)
+                if (16u * d < D) {
+                    const int32x4 z = {0, 0, 0, 0};
+                    const int32x4 c0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(vv[d], pd[0], z, 0, 0, 0);
+                    const int32x4 c1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(vv[d], pd[1], z, 0, 0, 0);
+                    const int32x4 c2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(vv[d], pd[2], z, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        o[d][i] += fmaf((float)c2[i], 65536.0f, (float)((c1[i] << 8) + c0[i])) * f;
+                }
         }
     }
     // the wavefronts' results joined
     const uint32_t row = D + 4;
-    float *lm = lds + DEC_W * 16 * NR * row;
-#pragma unroll
-    for (int n = 0; n < NR; n++) {
-        l[n] += __shfl_xor(l[n], 16);
-        l[n] += __shfl_xor(l[n], 32);
-        if (lane < 16) {
-            lm[(wave * NR + n) * 32 + lane] = m[n];
-            lm[(wave * NR + n) * 32 + 16 + lane] = l[n];
-        }
-        float *p = lds + ((wave * NR + n) * 16 + (lane & 15)) * row + 4 * g4;
-#pragma unroll
-        for (int d = 0; d < 4 * KS; d++)
-            if (16u * d < D) *(floatx4 *)(p + 16 * d) = o[n][d];
+    float *lm = lds + DEC_W * 16 * row;
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (lane < 16) {
+        lm[wave * 32 + lane] = m;
+        lm[wave * 32 + 16 + lane] = l;
     }
+    float *p = lds + (wave * 16 + (lane & 15)) * row + 4 * g4;
+#pragma unroll
+    for (int d = 0; d < 4 * KS; d++)
+        if (16u * d < D) *(floatx4 *)(p + 16 * d) = o[d];
     __syncthreads();
-    const uint32_t G = a.heads / a.c.heads, rows = min(a.tokens * G - at.rb * 16 * NR, 16u * NR);
+    const uint32_t n_rows = min(rows - r0, 16u * RB);
     const uint64_t seg = ((uint64_t)at.rb * a.s.count * a.c.heads + at.s * a.c.heads + at.kh) * a.splits + at.split;
-    for (uint32_t e = threadIdx.x; e < rows * (D / 4); e += DEC_NT) {
-        const uint32_t r = e / (D / 4), d = e % (D / 4) * 4, n = r / 16;
+    for (uint32_t e = threadIdx.x; e < n_rows * (D / 4); e += DEC_NT) {
+        const uint32_t r = e / (D / 4), d = e % (D / 4) * 4;
         float top = -__builtin_inff();
 #pragma unroll
-        for (uint32_t w = 0; w < DEC_W; w++) top = fmaxf(top, lm[(w * NR + n) * 32 + r % 16]);
+        for (uint32_t w = 0; w < PW; w++) top = fmaxf(top, lm[(w * RB + r / 16) * 32 + r % 16]);
         const float ref = top == -__builtin_inff() ? 0.0f : top;
         floatx4 sum = {0, 0, 0, 0};
         float ls = 0;
 #pragma unroll
-        for (uint32_t w = 0; w < DEC_W; w++) {
-            const float f = __builtin_amdgcn_exp2f(lm[(w * NR + n) * 32 + r % 16] - ref);
-            sum += *(const floatx4 *)(lds + ((w * NR + n) * 16 + r % 16) * row + d) * f;
-            ls += lm[(w * NR + n) * 32 + 16 + r % 16] * f;
+        for (uint32_t w = 0; w < PW; w++) {
+            const uint32_t n = w * RB + r / 16;
+            const float f = __builtin_amdgcn_exp2f(lm[n * 32 + r % 16] - ref);
+            sum += *(const floatx4 *)(lds + (n * 16 + r % 16) * row + d) * f;
+            ls += lm[n * 32 + 16 + r % 16] * f;
         }
-        if (a.splits > 1 || a.ml) {
-            if (d == 0) {
-                a.ml[(seg * 16 * NR + r) * 2] = top;
-                a.ml[(seg * 16 * NR + r) * 2 + 1] = ls;
-            }
+        sum *= 1.0f / DEC_P;
+        if (a.ml && d == 0) {
+            a.ml[(seg * 16 * RB + r) * 2] = top;
+            a.ml[(seg * 16 * RB + r) * 2 + 1] = ls;
         }
         if (a.splits > 1) {
-            *(floatx4 *)(a.part + (seg * 16 * NR + r) * D + d) = sum;
+            *(floatx4 *)(a.part + (seg * 16 * RB + r) * D + d) = sum;
         } else {
-            const uint32_t rr = at.rb * 16 * NR + r;
+            const uint32_t rr = r0 + r;
             float *out = a.o + (((uint64_t)at.s * a.tokens + rr / G) * a.heads + at.kh * G + rr % G) * D + d;
-            *(floatx4 *)out = ls != 0 ? sum * (1.0f / (ls * DEC_P)) : floatx4{0, 0, 0, 0};
+            *(floatx4 *)out = ls != 0 ? sum * (1.0f / ls) : floatx4{0, 0, 0, 0};
         }
     }
 }
 
-// Visible pages of a block of rows, as its first and last row see them.
-__device__ __forceinline__ uint2 dec_block_pages(const DecArgs &a, uint32_t s, uint32_t r0, uint32_t r1) {
-    const uint32_t G = a.heads / a.c.heads;
-    const int64_t len = max(a.s.len[s], 0);
-    const uint32_t cap = (uint32_t)min(len, (int64_t)a.s.stride * KV_B);
-    const int64_t e0 = max(len - a.tokens + r0 / G + 1, (int64_t)0), e1 = max(len - a.tokens + r1 / G + 1, (int64_t)0);
-    return dec_pages(a.window && e0 > a.window ? (uint32_t)(e0 - a.window) : 0, (uint32_t)min(e1, (int64_t)cap));
-}
-
-// Joins the splits: one workgroup a query row (query token and head); threads
-// take four dimensions of every (1024 / dim)-th split each.
+// Joins the splits: one workgroup a query row (query token and head).  The splits'
+// factors first, a thread each; then threads take four dimensions of every (1024 /
+// dim)-th split, four of them under way.
+constexpr uint32_t DEC_SPLITS = 1024;
 __global__ __launch_bounds__(DEC_NT) void attn_dec_join_kernel(DecArgs a, uint32_t rpb) {
     __shared__ __align__(16) float acc[DEC_NT * 4];
+    __shared__ float w[DEC_SPLITS], red[2 * DEC_W];
     const uint32_t G = a.heads / a.c.heads, rows = a.tokens * G, D = a.c.dim, tid = threadIdx.x;
     const uint32_t r = blockIdx.x % rows, sh = blockIdx.x / rows, s = sh / a.c.heads, kh = sh % a.c.heads;
     const uint32_t rb = r / rpb, r0 = rb * rpb;
     const uint2 pg = dec_block_pages(a, s, r0, min(r0 + rpb, rows) - 1);
     const uint32_t chunk = dec_chunk(pg, a.splits), ns = chunk ? (pg.y - pg.x + chunk - 1) / chunk : 0;
     const uint64_t seg = ((uint64_t)rb * a.s.count * a.c.heads + sh) * a.splits;
-    const float *ml = a.ml + (seg * rpb + (r - r0)) * 2;
-    const uint64_t step = (uint64_t)rpb * 2;
-    float top = -__builtin_inff();
-    for (uint32_t i = 0; i < ns; i++) top = fmaxf(top, ml[i * step]);
+    const float2 *ml = (const float2 *)a.ml + seg * rpb + (r - r0);
+    float2 x[DEC_SPLITS / DEC_NT];
+    float top = -__builtin_inff(), ls = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < DEC_SPLITS / DEC_NT; i++) {
+        const uint32_t j = tid + i * DEC_NT;
+        x[i] = j < ns ? ml[(uint64_t)j * rpb] : float2{-__builtin_inff(), 0};
+        top = fmaxf(top, x[i].x);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    if ((tid & 63) == 0) red[tid >> 6] = top;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < DEC_W; i++) top = fmaxf(top, red[i]);
     const float ref = top == -__builtin_inff() ? 0.0f : top;
+#pragma unroll
+    for (uint32_t i = 0; i < DEC_SPLITS / DEC_NT; i++) {
+        const float f = __builtin_amdgcn_exp2f(x[i].x - ref);
+        w[tid + i * DEC_NT] = f;
+        ls += x[i].y * f;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) ls += __shfl_xor(ls, o);
+    if ((tid & 63) == 0) red[DEC_W + (tid >> 6)] = ls;
+    __syncthreads();
+    ls = red[DEC_W];
+#pragma unroll
+    for (uint32_t i = 1; i < DEC_W; i++) ls += red[DEC_W + i];
     const uint32_t q4 = D / 4, groups = DEC_NT / q4, g = tid / q4, d = tid % q4 * 4;
     floatx4 sum = {0, 0, 0, 0};
-    float ls = 0;
-    if (g < groups)
-        for (uint32_t i = g; i < ns; i += groups) {
-            const float f = __builtin_amdgcn_exp2f(ml[i * step] - ref);
-            ls += ml[i * step + 1] * f;
-            sum += *(const floatx4 *)(a.part + ((seg + i) * rpb + (r - r0)) * D + d) * f;
+    if (g < groups) {
+        const float *part = a.part + (seg * rpb + (r - r0)) * D + d;
+        for (uint32_t i = g; i < ns; i += 4 * groups) {
+            floatx4 y[4];
+#pragma unroll
+            for (uint32_t u = 0; u < 4; u++) y[u] = *(const floatx4 *)(part + (uint64_t)min(i + u * groups, ns - 1) * rpb * D);
+#pragma unroll
+            for (uint32_t u = 0; u < 4; u++)
+                if (i + u * groups < ns) sum += y[u] * w[i + u * groups];
         }
+    }
     *(floatx4 *)(acc + tid * 4) = sum;
     __syncthreads();
-    __shared__ float lsum[DEC_NT];
-    lsum[tid] = g < groups ? ls : 0;
-    __syncthreads();
     if (tid < q4) {
-        for (uint32_t i = 1; i < groups; i++) {
-            sum += *(const floatx4 *)(acc + (i * q4 + tid) * 4);
-            ls += lsum[i * q4 + tid];
-        }
+        for (uint32_t i = 1; i < groups; i++) sum += *(const floatx4 *)(acc + (i * q4 + tid) * 4);
         float *out = a.o + (((uint64_t)s * a.tokens + r / G) * a.heads + kh * G + r % G) * D + d;
-        *(floatx4 *)out = ls != 0 ? sum * (1.0f / (ls * DEC_P)) : floatx4{0, 0, 0, 0};
+        *(floatx4 *)out = ls != 0 ? sum * (1.0f / ls) : floatx4{0, 0, 0, 0};
     }
+}
+
+// x of the lane N before this one in its row of 16, around.
+template <int N>
+__device__ __forceinline__ float dec_ror(float x) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), 0x120 + N, 0xF, 0xF, false));
 }
 
 // Accumulated attention weights: a wavefront a page, the scores computed again
@@ -425,37 +464,53 @@ __global__ __launch_bounds__(DEC_NT, KS <= 2 ? 2 : 1) void attn_dec_weights_kern
             ls += __shfl_xor(ls, 32);
             inv[n] = valid && ls != 0 ? 1.0f / ls : 0.0f;
         }
-        for (uint32_t p = part * chunk + wave; p < min((part + 1) * chunk, np); p += DEC_W) {
-            const uint32_t j0 = p * KV_B;
-            const int32_t id = pages[p];
-            const uint32_t j = j0 + lane;
-            float w = 0;
-            if ((uint32_t)id < a.c.pages && j0 < q.hi_max && j0 + KV_B > q.lo_min) {
-                const uint64_t ph = (uint64_t)id * a.c.heads + kh;
-                int32x4 kk[4][KS];
-                dec_load_k<KS>(kk, a.c.k + ph * KV_B * D, D);
-                float sc[NR][16], sum[16];
-                dec_scores<KS, NR>(sc, kk, q, a.c.ks[ph], j0);
+        const uint32_t p1 = min((part + 1) * chunk, np);
+        for (uint32_t b = part * chunk + wave; b < p1; b += 64 * DEC_W) {
+            // page ids and scales of this wavefront's next 64 pages, one a lane
+            const uint32_t mine = b + lane * DEC_W, pages_here = min((p1 - b + DEC_W - 1) / DEC_W, 64u);
+            const int32_t id = mine < p1 ? pages[mine] : -1;
+            const bool have = (uint32_t)id < a.c.pages && mine * KV_B < q.hi_max && mine * KV_B + KV_B > q.lo_min;
+            const uint64_t ph = have ? (uint64_t)id * a.c.heads + kh : 0;
+            const float lks = have ? a.c.ks[ph] : 0;
+            const uint64_t live = __ballot(have);
+            auto keys = [&](int32x4 (&kk)[4][KS], uint32_t u) {
+                if (u >= pages_here || !(live >> u & 1)) return;
+                const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(ph >> 32), u) << 32 | (uint32_t)__builtin_amdgcn_readlane((uint32_t)ph, u);
+                dec_load_k<KS>(kk, a.c.k + at * KV_B * D, D);
+            };
+            int32x4 kk[4][KS];
+            keys(kk, 0);
+            for (uint32_t u = 0; u < pages_here; u++) {
+                // lane (g, r) has the token 16 (r / 4) + 4 g + r % 4 of the page
+                const uint32_t j0 = (b + u * DEC_W) * KV_B, r = lane & 15, j = j0 + 16 * (r / 4) + 4 * g4 + r % 4;
+                const bool here = j < cap;
+                const float was = !here ? 0.0f : rb ? wo[j] : wi ? wi[j] : 0.0f;
+                float w = 0;
+                if (live >> u & 1) {
+                    float sc[NR][16];
+                    dec_scores<KS, NR>(sc, kk, q, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lks), u)), j0);
+                    keys(kk, u + 1);
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    sum[i] = 0;
+                    for (int i = 0; i < 16; i++) {
+                        float sum = 0;
 #pragma unroll
-                    for (int n = 0; n < NR; n++) {
-                        const float e = __builtin_amdgcn_exp2f(sc[n][i] - ref[n]) * inv[n];
-                        // (unseen tokens get nothing of a row whose sum is NaN)
-                        sum[i] += rb * 16 * NR + 16 * n + (lane & 15) < rows && sc[n][i] != -__builtin_inff() ? e : 0.0f;
+                        for (int n = 0; n < NR; n++) {
+                            const float e = __builtin_amdgcn_exp2f(sc[n][i] - ref[n]) * inv[n];
+                            // (unseen tokens get nothing of a row whose sum is NaN; rows that are not there count 0)
+                            sum += inv[n] != 0 && sc[n][i] != -__builtin_inff() ? e : 0.0f;
+                        }
+                        // the sixteen lanes of the group added up, in all of them
+                        sum += dec_ror<8>(sum);
+                        sum += dec_ror<4>(sum);
+                        sum += dec_ror<2>(sum);
+                        sum += dec_ror<1>(sum);
+                        w = (int)r == i ? sum : w;
                     }
-#pragma unroll
-                    for (int x = 1; x < 16; x <<= 1) sum[i] += __shfl_xor(sum[i], x);
+                } else {
+                    keys(kk, u + 1);
                 }
-                // token lane = 16 t + 4 g + i is held by lanes of group g, at 4 t + i
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const float v = __shfl(sum[i], (lane >> 2 & 3) * 16);
-                    if ((lane >> 4) == i / 4 && (lane & 3) == i % 4) w = v;
-                }
+                if (here) wo[j] = was + w;
             }
-            if (j < cap) wo[j] = (rb ? wo[j] : wi ? wi[j] : 0.0f) + w;
         }
     }
 }
