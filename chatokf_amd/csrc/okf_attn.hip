@@ -71,7 +71,7 @@ int check_rows(const okf_kv_cache *c, const okf_kv_seqs *s, const void *k, const
     const uint64_t row = (uint64_t)c->heads * c->dim;
     if (!row_stride(ks, row, size) || !row_stride(vs, row, size)) return OKF_E_SHAPE;
     const uint64_t items = n / KV_B + 3ull * s->count;
-    if (items > 0x7FFFFFFFull) return OKF_E_SHAPE;
+    if (items > 0xFFFFFFull) return OKF_E_SHAPE;  // (a grid has less than 2^32 threads)
     grid = dim3((uint32_t)items, c->heads, 2);
     return OKF_OK;
 }
@@ -103,7 +103,7 @@ int plan_decode(okf_ctx *c, DecArgs &a) {
         a.ml = c->part;
         a.part = c->part + base * splits * rpb * 2;
     }
-    if ((base * splits + 8 * a.rb) > 0x7FFFFFFFull) return OKF_E_SHAPE;
+    if (base * splits + 8ull * a.rb > 0xFFFFFFull) return OKF_E_SHAPE;
     return OKF_OK;
 }
 
@@ -114,12 +114,12 @@ void launch_decode_n(okf_ctx *c, const DecArgs &a) {
     const uint32_t sh = a.s.count * a.c.heads;
     const size_t lds = (size_t)DEC_W * 16 * (a.c.dim + 4 + 2) * sizeof(float);
     hipLaunchKernelGGL((attn_dec_kernel<KS, NR>), dim3((sh * a.splits + 7) / 8 * 8 * a.rb), dim3(DEC_NT), lds, c->stream, a);
-    if (a.splits > 1)
-        hipLaunchKernelGGL(attn_dec_join_kernel, dim3(sh * a.tokens * (a.heads / a.c.heads)), dim3(DEC_NT), 0, c->stream, a,
-                           16u * NR);
+    const uint32_t joins = a.splits > 1 ? sh * a.tokens * (a.heads / a.c.heads) : 0;
     if (a.w_out) {
         const uint32_t parts = std::max(1u, std::min(4 * c->cus / sh, (a.s.stride + DEC_W - 1) / DEC_W));
-        hipLaunchKernelGGL((attn_dec_weights_kernel<KS, NR>), dim3(sh * parts), dim3(DEC_NT), 0, c->stream, a, parts);
+        hipLaunchKernelGGL((attn_dec_weights_kernel<KS, NR>), dim3(joins + sh * parts), dim3(DEC_NT), 0, c->stream, a, parts, joins);
+    } else if (joins) {
+        hipLaunchKernelGGL(attn_dec_join_kernel, dim3(joins), dim3(DEC_NT), 0, c->stream, a, 16u * NR);
     }
 }
 
@@ -231,7 +231,7 @@ int okf_kv_evict(okf_ctx *c, const okf_kv_cache *src, const okf_kv_seqs *from, c
     if (w_in_stride < (uint64_t)from->stride * KV_B || (w_out && w_out_stride < keep)) return OKF_E_SHAPE;
     if (!aligned4(w_in) || !aligned4(w_out) || !aligned4(kept)) return OKF_E_SHAPE;
     const uint64_t rows = (uint64_t)from->count * src->heads;
-    if (rows > 0x7FFFFFFFull) return OKF_E_SHAPE;
+    if (rows > 0x3FFFFFull || keep > 0x3FFFFFFFu) return OKF_E_SHAPE;  // (grids of less than 2^32 threads)
     // (the second grid: sequences over y, in groups that fit it, and z)
     const uint32_t group = std::min(from->count, 65535 / src->heads);
     const uint32_t groups = (from->count + group - 1) / group;

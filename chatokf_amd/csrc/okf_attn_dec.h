@@ -360,7 +360,7 @@ __global__ __launch_bounds__(DEC_NT, KS <= 2 ? 2 : 1) void attn_dec_kernel(DecAr
 // factors first, a thread each; then threads take four dimensions of every (1024 /
 // dim)-th split, four of them under way.
 constexpr uint32_t DEC_SPLITS = 1024;
-__global__ __launch_bounds__(DEC_NT) void attn_dec_join_kernel(DecArgs a, uint32_t rpb) {
+__device__ __forceinline__ void dec_join(const DecArgs &a, uint32_t rpb) {
     __shared__ __align__(16) float acc[DEC_NT * 4];
     __shared__ float w[DEC_SPLITS], red[2 * DEC_W];
     const uint32_t G = a.heads / a.c.heads, rows = a.tokens * G, D = a.c.dim, tid = threadIdx.x;
@@ -420,6 +420,8 @@ __global__ __launch_bounds__(DEC_NT) void attn_dec_join_kernel(DecArgs a, uint32
     }
 }
 
+__global__ __launch_bounds__(DEC_NT) void attn_dec_join_kernel(DecArgs a, uint32_t rpb) { dec_join(a, rpb); }
+
 // x of the lane N before this one in its row of 16, around.
 template <int N>
 __device__ __forceinline__ float dec_ror(float x) {
@@ -430,9 +432,11 @@ __device__ __forceinline__ float dec_ror(float x) {
 // from the keys, for every block of query rows.  (Stored scores would be 8 bytes a
 // token and query row, and scratch of the cache's capacity.)
 template <int KS, int NR>
-__global__ __launch_bounds__(DEC_NT, KS <= 2 ? 2 : 1) void attn_dec_weights_kernel(DecArgs a, uint32_t parts) {
+__global__ __launch_bounds__(DEC_NT, KS <= 2 ? 2 : 1) void attn_dec_weights_kernel(DecArgs a, uint32_t parts, uint32_t joins) {
+    if (blockIdx.x < joins) return dec_join(a, 16 * NR);  // (the splits' results beside them)
+    const uint32_t id_ = blockIdx.x - joins;
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, D = a.c.dim, g4 = lane >> 4;
-    const uint32_t sh = blockIdx.x / parts, s = sh / a.c.heads, kh = sh % a.c.heads, part = blockIdx.x % parts;
+    const uint32_t sh = id_ / parts, s = sh / a.c.heads, kh = sh % a.c.heads, part = id_ % parts;
     const uint32_t cap = (uint32_t)min((uint64_t)max(a.s.len[s], 0), (uint64_t)a.s.stride * KV_B);
     const uint32_t np = (cap + KV_B - 1) / KV_B, chunk = (np + parts - 1) / parts;
     const uint32_t rows = a.tokens * (a.heads / a.c.heads);
