@@ -186,9 +186,19 @@ __global__ __launch_bounds__(S::NT, S::WAVES) void attn_prompt_kernel(AttnArgs a
     extern __shared__ __align__(16) uint8_t at_mem[];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), D = DH ? DH : a.dim;
     const uint32_t rg = wave % RG, kg = wave / RG, h = lane >> 5;
-    // heads of one kv head on one XCD where they divide over the eight
-    uint32_t head = blockIdx.x % a.heads;
-    const SeqItem it = at_tile<BM>(a, blockIdx.x / a.heads);
+    // A kv head's workgroups on as few XCDs (workgroups a multiple of 8 apart) as there are for
+    // it, tiles in order: kv heads that divide 8 have 8 / kv_heads XCDs each; else heads that 8
+    // divides lie side by side on one.
+    uint32_t head = blockIdx.x % a.heads, rank = blockIdx.x / a.heads;
+    if (8 % a.kv_heads == 0) {
+        const uint32_t x = blockIdx.x % 8, group = a.heads / a.kv_heads;
+        const uint32_t at = blockIdx.x / 8 * (8 / a.kv_heads) + x / a.kv_heads;
+        head = x % a.kv_heads * group + at % group;
+        rank = at / group;
+    } else if (a.heads % 8 == 0) {
+        head = head % 8 * (a.heads / 8) + head / 8;
+    }
+    const SeqItem it = at_tile<BM>(a, rank);
     if (it.seq >= a.seqs) return;
     const uint2 rq = kv_rows(a.q_start, it.seq, a.nq), rk = kv_rows(a.k_start, it.seq, a.nk);
     const int nq = rq.y - rq.x, nk = rk.y - rk.x, i0 = it.at * BM, w = (int)min(a.window, 0x7FFFFFFFu);

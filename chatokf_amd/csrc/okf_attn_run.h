@@ -11,11 +11,16 @@ int launch_prompt_s(okf_ctx *c, okf::AttnArgs a) {
     using namespace okf;
     // (sequences' tiles: at most n_q / rows and one each; never more than the rows)
     const uint64_t tiles = std::min<uint64_t>((uint64_t)a.nq / S::BM + a.seqs, a.nq);
-    if (tiles * a.heads > 0xFFFFFFull) return OKF_E_SHAPE;  // (a grid has less than 2^32 threads)
+    uint64_t grid = tiles * a.heads;
+    if (8 % a.kv_heads == 0) {  // (as the kernel deals them to the XCDs)
+        const uint64_t each = 8 / a.kv_heads;
+        grid = (tiles * (a.heads / a.kv_heads) + each - 1) / each * 8;
+    }
+    if (grid * S::NT > 0xFFFFFFFFull) return OKF_E_SHAPE;  // (a grid has less than 2^32 threads)
     a.tiles = (uint32_t)tiles;
     static std::atomic<uint64_t> attr{0};
     set_lds_attr(c, (const void *)attn_prompt_kernel<T, S>, attr);
-    hipLaunchKernelGGL((attn_prompt_kernel<T, S>), dim3(a.tiles * a.heads), dim3(S::NT), (at_lds<S>()), c->stream, a);
+    hipLaunchKernelGGL((attn_prompt_kernel<T, S>), dim3((uint32_t)grid), dim3(S::NT), (at_lds<S>()), c->stream, a);
     return OKF_OK;
 }
 
