@@ -82,6 +82,7 @@ int check_rows(const okf_kv_cache *c, const okf_kv_seqs *s, const void *k, const
 // workgroup's wavefronts; batches of ragged sequences get twice that, so that the
 // short ones' workgroups make room for the long ones'.  The partial results go to
 // the context's buffer; where it may not grow, as many splits as it holds.
+constexpr uint64_t DEC_KEPT = 256ull << 20;  // bytes of scores at most
 int plan_decode(okf_ctx *c, DecArgs &a) {
     const uint64_t rows = (uint64_t)a.tokens * (a.heads / a.c.heads), rpb = rows > 16 ? 32 : 16;
     a.rb = (uint32_t)((rows + rpb - 1) / rpb);
@@ -92,7 +93,14 @@ int plan_decode(okf_ctx *c, DecArgs &a) {
     auto bytes = [&](uint64_t n) {  // m and l, then partial outputs
         return base * n * rpb * 2 * sizeof(float) + (n > 1 ? base * n * rpb * a.c.dim * sizeof(float) : 0);
     };
-    if (splits > 1 || a.w_out) {
+    // Scores kept for the weights, where that is less to write and read than the keys are to read
+    // again (8 sequences of up to 16000 tokens, 2 rows of 64: 31.6 us without) and the room is there.
+    const uint64_t kept = a.w_out && a.rb == 1 && rpb == 16 && 8 * rows <= a.c.dim
+                              ? base * rows * a.s.stride * KV_B * sizeof(float) : 0;
+    const uint64_t to = (bytes(splits) + 15) / 16 * 16;
+    if (kept && kept <= DEC_KEPT && (to + kept <= c->part_bytes || grow_part(c, to + kept, true) == OKF_OK))
+        a.sc = c->part + to / sizeof(float);
+    else if (splits > 1 || a.w_out) {
         if (bytes(splits) > c->part_bytes && grow_part(c, bytes(splits), true) != OKF_OK) {
             while (splits > 1 && bytes(splits) > c->part_bytes) splits--;
             if (a.w_out && bytes(splits) > c->part_bytes) return OKF_E_SHAPE;
@@ -115,7 +123,10 @@ void launch_decode_n(okf_ctx *c, const DecArgs &a) {
     const size_t lds = (size_t)DEC_W * 16 * (a.c.dim + 4 + 2) * sizeof(float);
     hipLaunchKernelGGL((attn_dec_kernel<KS, NR>), dim3((sh * a.splits + 7) / 8 * 8 * a.rb), dim3(DEC_NT), lds, c->stream, a);
     const uint32_t joins = a.splits > 1 ? sh * a.tokens * (a.heads / a.c.heads) : 0;
-    if (a.w_out) {
+    if (a.sc) {
+        const uint32_t parts = std::max(1u, std::min(8 * c->cus / sh, (a.s.stride * KV_B + DEC_NT - 1) / DEC_NT));
+        hipLaunchKernelGGL(attn_dec_sum_kernel, dim3(joins + sh * parts), dim3(DEC_NT), 0, c->stream, a, parts, joins);
+    } else if (a.w_out) {
         const uint32_t parts = std::max(1u, std::min(4 * c->cus / sh, (a.s.stride + DEC_W - 1) / DEC_W));
         hipLaunchKernelGGL((attn_dec_weights_kernel<KS, NR>), dim3(joins + sh * parts), dim3(DEC_NT), 0, c->stream, a, parts, joins);
     } else if (joins) {
@@ -175,7 +186,7 @@ int okf_attn_decode(okf_ctx *c, const okf_kv_cache *cache, const okf_kv_seqs *se
     if (sh * rows > 0x3FFFFFFFull) return OKF_E_SHAPE;
     if ((st = begin(c))) return st;
     DecArgs a{cache_of(cache), seqs_of(seqs), q, o, tokens, heads, scale, window, w_in, w_out, w_stride, 1, 1,
-              nullptr, nullptr};
+              nullptr, nullptr, nullptr};
     if ((st = plan_decode(c, a))) return st;
     if (a.ml) note_capture(c, false, true, false);
     with_dims(cache->dim, [&](auto ks) { launch_decode<decltype(ks)::value>(c, a, rows > 16); });

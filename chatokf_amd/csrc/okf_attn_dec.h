@@ -50,6 +50,7 @@ struct DecArgs {
     uint64_t wst;
     uint32_t splits, rb;   // page ranges a sequence; blocks of 16 NR query rows
     float *part, *ml;      // [row block][split][16 NR][dim], [row block][split][16 NR][2]
+    float *sc;             // scores [sequence][kv head][row][64 stride] for the weights, or null: they are made again
 };
 
 // Four integers + 0x808080 -> the dwords of their three digit planes.
@@ -263,6 +264,11 @@ __global__ __launch_bounds__(DEC_NT, KS <= 2 ? 2 : 1) void attn_dec_kernel(DecAr
                 off = base(at_lane);
                 dec_load_k<KS>(kk, a.c.k + off, D);
             }
+            if (RB == 1 && a.sc && (lane & 15) < rows) {
+                float *to = a.sc + (((uint64_t)at.s * a.c.heads + at.kh) * rows + (lane & 15)) * ((uint64_t)a.s.stride * KV_B) + j0 + 4 * g4;
+#pragma unroll
+                for (int t = 0; t < 4; t++) *(floatx4 *)(to + 16 * t) = floatx4{s[0][4 * t], s[0][4 * t + 1], s[0][4 * t + 2], s[0][4 * t + 3]};
+            }
             float x = s[0][0];
 #pragma unroll
             for (int i = 1; i < 16; i++) x = fmaxf(x, s[0][i]);
@@ -428,9 +434,50 @@ __device__ __forceinline__ float dec_ror(float x) {
     return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), 0x120 + N, 0xF, 0xF, false));
 }
 
+// Accumulated attention weights from the scores that attn_dec_kernel has left (up to 16
+// query rows): the rows' maxima and sums over the splits first, a wavefront a row, then a
+// thread a token.
+__global__ __launch_bounds__(DEC_NT) void attn_dec_sum_kernel(DecArgs a, uint32_t parts, uint32_t joins) {
+    if (blockIdx.x < joins) return dec_join(a, 16);  // (the splits' results beside them)
+    __shared__ float top_of[16], inv_of[16];
+    const uint32_t id_ = blockIdx.x - joins, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t sh = id_ / parts, s = sh / a.c.heads, part = id_ % parts;
+    const uint32_t cap = (uint32_t)min((uint64_t)max(a.s.len[s], 0), (uint64_t)a.s.stride * KV_B);
+    const uint32_t rows = a.tokens * (a.heads / a.c.heads);
+    const uint2 pg = dec_block_pages(a, s, 0, rows - 1);
+    const uint32_t ch = dec_chunk(pg, a.splits), ns = ch ? (pg.y - pg.x + ch - 1) / ch : 0;
+    for (uint32_t r = wave; r < rows; r += DEC_W) {
+        const float2 *ml = (const float2 *)a.ml + (uint64_t)sh * a.splits * 16 + r;
+        float top = -__builtin_inff(), ls = 0;
+        for (uint32_t i = lane; i < ns; i += 64) top = fmaxf(top, ml[i * 16].x);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+        const float ref = top == -__builtin_inff() ? 0.0f : top;
+        for (uint32_t i = lane; i < ns; i += 64) ls += ml[i * 16].y * __builtin_amdgcn_exp2f(ml[i * 16].x - ref);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) ls += __shfl_xor(ls, o);
+        if (lane == 0) top_of[r] = ref, inv_of[r] = ls != 0 ? 1.0f / ls : 0.0f;
+    }
+    __syncthreads();
+    const uint64_t row = (uint64_t)a.s.stride * KV_B;
+    const int32_t *pages = a.s.pages + (uint64_t)s * a.s.stride;
+    const float *sc = a.sc + (uint64_t)sh * rows * row, *wi = a.w_in ? a.w_in + (uint64_t)sh * a.wst : nullptr;
+    float *wo = a.w_out + (uint64_t)sh * a.wst;
+    for (uint64_t j = part * DEC_NT + threadIdx.x; j < cap; j += (uint64_t)parts * DEC_NT) {
+        const uint32_t p = j / KV_B;
+        float w = 0;
+        if ((uint32_t)pages[p] < a.c.pages && p >= pg.x && p < pg.y)
+            for (uint32_t r = 0; r < rows; r++) {
+                const float x = sc[r * row + j];
+                // (unseen tokens get nothing of a row whose sum is NaN)
+                w += x != -__builtin_inff() ? __builtin_amdgcn_exp2f(x - top_of[r]) * inv_of[r] : 0.0f;
+            }
+        wo[j] = (wi ? wi[j] : 0.0f) + w;
+    }
+}
+
 // Accumulated attention weights: a wavefront a page, the scores computed again
-// from the keys, for every block of query rows.  (Stored scores would be 8 bytes a
-// token and query row, and scratch of the cache's capacity.)
+// from the keys, for every block of query rows: where the scores have not been kept.
 template <int KS, int NR>
 __global__ __launch_bounds__(DEC_NT, KS <= 2 ? 2 : 1) void attn_dec_weights_kernel(DecArgs a, uint32_t parts, uint32_t joins) {
     if (blockIdx.x < joins) return dec_join(a, 16 * NR);  // (the splits' results beside them)

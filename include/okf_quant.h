@@ -329,9 +329,11 @@ int okf_kv_read(okf_ctx *ctx, const okf_kv_cache *cache, const okf_kv_seqs *seqs
  * token got is added up: w_out[s][head][t] = w_in[s][head][t] + the sum over
  * the queries and the query heads of the kv head, t < len, rows of w_stride
  * values; w_in NULL counts as 0, w_in = w_out adds in place.
- * Scratch: the partial results of sequences split over workgroups, in the
- * context's buffer (see okf_ctx_reserve); where it may not grow, fewer splits
- * (the order of the fp32 sums changes). */
+ * Scratch: the partial results of sequences split over workgroups, and with w_out
+ * and few rows the scores (at most 256 MB; else they are computed twice), in the
+ * context's buffer (see okf_ctx_reserve); where it may not grow, fewer splits and
+ * no scores (the order of the fp32 sums changes), and with w_out OKF_E_SHAPE if
+ * not even one split fits. */
 int okf_attn_decode(okf_ctx *ctx, const okf_kv_cache *cache, const okf_kv_seqs *seqs, const float *q, float *o,
                     uint32_t tokens, uint32_t heads, float scale, uint32_t window, const float *w_in, float *w_out,
                     uint64_t w_stride);
