@@ -406,9 +406,9 @@ __global__ __launch_bounds__(EV_NT) void kv_select_kernel(KvSeqs from, int32_t *
         }
         return;
     }
+    // The tokens that stay anyway have keys above all weights', so that the `keep` largest are
+    // looked for; places past the end have 0 and come last among those (NaN) of 0.
     const uint32_t lo = sink, hi = len - recent;
-    uint32_t want = keep - sink - recent;  // of [lo, hi)
-    const bool none = want == 0;
     // tokens of a wavefront, in 64s; this lane's first one of a round of EV_ALL
     const uint32_t per = min((len + EV_NT - 1) / EV_NT, EV_PER), mine = tid / 64 * 64 * per + lane;
     uint32_t k[EV_PER];
@@ -416,61 +416,57 @@ __global__ __launch_bounds__(EV_NT) void kv_select_kernel(KvSeqs from, int32_t *
 #pragma unroll
         for (uint32_t u = 0; u < EV_PER; u++) {
             const uint32_t i = b + mine + u * 64;
-            k[u] = u < per && i < len ? kv_key(w[i]) : 0;
+            k[u] = u < per && i < len ? (i >= lo && i < hi ? kv_key(w[i]) : 0xFFFFFFFFu) : 0;
         }
     };
-    auto inner = [&](uint32_t i) { return i >= lo && i < hi; };
+    auto below = [](uint64_t who) { return __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0)); };
     load(0);
-    uint32_t key = 0, mask = 0;
-    if (!none) {
+    uint32_t want = keep, key = 0, mask = 0;
 #pragma unroll 1
-        for (int round = 0; round < 3; round++) {
-            const uint32_t shift = round == 0 ? 21 : round == 1 ? 10 : 0, bits = round == 2 ? 1023 : 2047;
-            hist[tid] = hist[tid + EV_NT] = 0;
-            __syncthreads();
-            for (uint32_t b = 0; b < len; b += EV_ALL) {
-                if (len > EV_ALL) load(b);
+    for (int round = 0; round < 3; round++) {
+        const uint32_t shift = round == 0 ? 21 : round == 1 ? 10 : 0, bits = round == 2 ? 1023 : 2047;
+        hist[tid] = hist[tid + EV_NT] = 0;
+        __syncthreads();
+        for (uint32_t b = 0; b < len; b += EV_ALL) {
+            if (len > EV_ALL) load(b);
 #pragma unroll
-                for (uint32_t u = 0; u < EV_PER; u++) {
-                    if (u < per) {
-                        const bool in = inner(b + mine + u * 64) && (k[u] & mask) == key;
-                        const uint64_t who = __ballot(in);
-                        if (who) {
-                            const uint32_t d = k[u] >> shift & bits;
-                            const int first = __ffsll((unsigned long long)who) - 1;
-                            const uint32_t d0 = __builtin_amdgcn_readlane(d, first);
-                            // (all in one bin, as equal weights are: one addition)
-                            if (__ballot(in && d == d0) == who) {
-                                if ((int)lane == first) atomicAdd(&hist[d0], (uint32_t)__popcll(who));
-                            } else if (in) {
-                                atomicAdd(&hist[d], 1u);
-                            }
+            for (uint32_t u = 0; u < EV_PER; u++)
+                if (u < per) {
+                    const bool in = (k[u] & mask) == key;
+                    const uint64_t who = __ballot(in);
+                    if (who) {
+                        const uint32_t d = k[u] >> shift & bits;
+                        const int first = __ffsll((unsigned long long)who) - 1;
+                        const uint32_t d0 = __builtin_amdgcn_readlane(d, first);
+                        // (all in one bin, as equal weights are: one addition)
+                        if (__ballot(in && d == d0) == who) {
+                            if ((int)lane == first) atomicAdd(&hist[d0], (uint32_t)__popcll(who));
+                        } else if (in) {
+                            atomicAdd(&hist[d], 1u);
                         }
                     }
                 }
-            }
-            __syncthreads();
-            // the digit at which the count from the top reaches `want`: two a thread
-            const bool on = 2 * tid < bits;
-            const uint32_t top = bits - 2 * tid, h0 = on ? hist[top] : 0, h1 = on ? hist[top - 1] : 0;
-            uint32_t total;
-            const uint32_t upto = block_scan<EV_NT>(h0 + h1, red, total), before = upto - h0 - h1;
-            if (upto >= want && before < want) {
-                const bool one = before + h0 >= want;
-                pick[0] = one ? top : top - 1;
-                pick[1] = want - before - (one ? 0 : h0);
-            }
-            __syncthreads();
-            key |= pick[0] << shift;
-            mask |= bits << shift;
-            want = pick[1];
         }
+        __syncthreads();
+        // the digit at which the count from the top reaches `want`: two a thread
+        const bool on = 2 * tid < bits;
+        const uint32_t top = bits - 2 * tid, h0 = on ? hist[top] : 0, h1 = on ? hist[top - 1] : 0;
+        uint32_t total;
+        const uint32_t upto = block_scan<EV_NT>(h0 + h1, red, total), before = upto - h0 - h1;
+        if (upto >= want && before < want) {
+            const bool one = before + h0 >= want;
+            pick[0] = one ? top : top - 1;
+            pick[1] = want - before - (one ? 0 : h0);
+        }
+        __syncthreads();
+        key |= pick[0] << shift;
+        mask |= bits << shift;
+        want = pick[1];
     }
-    // in order: larger keys, the first `want` of equal ones, sink and recent
+    // in order: larger keys and the first `want` of equal ones
     uint32_t at = 0, ties = 0;
     for (uint32_t b = 0; b < len; b += EV_ALL) {
         if (len > EV_ALL) load(b);
-        auto below = [&](uint64_t who) { return (uint32_t)__popcll(who & ((1ull << lane) - 1)); };
         // what a wavefront has, from `have`, to what all have before it
         auto share = [&](uint32_t have, uint32_t &all) {
             __syncthreads();
@@ -488,38 +484,41 @@ __global__ __launch_bounds__(EV_NT) void kv_select_kernel(KvSeqs from, int32_t *
         uint32_t nt = 0, ns = 0, all;
 #pragma unroll
         for (uint32_t u = 0; u < EV_PER; u++)
-            if (u < per) nt += __popcll(__ballot(!none && inner(b + mine + u * 64) && k[u] == key));
+            if (u < per) nt += __popcll(__ballot(k[u] == key));
         uint32_t tie = ties + share(nt, all);
         ties += all;
         uint32_t stays = 0;  // bit u: token u stays
 #pragma unroll
-        for (uint32_t u = 0; u < EV_PER; u++) {
+        for (uint32_t u = 0; u < EV_PER; u++)
             if (u < per) {
-                const uint32_t i = b + mine + u * 64;
-                const bool eq = !none && inner(i) && k[u] == key;
-                const uint64_t who = __ballot(eq);
-                const bool stay = i < len && (!inner(i) || (!none && (k[u] > key || (eq && tie + below(who) < want))));
-                tie += __popcll(who);
+                const uint64_t who = __ballot(k[u] == key);
+                bool stay = k[u] > key;
+                if (who) {
+                    stay |= k[u] == key && tie + below(who) < want;
+                    tie += __popcll(who);
+                }
                 stays |= (uint32_t)stay << u;
                 ns += __popcll(__ballot(stay));
             }
-        }
         uint32_t to = at + share(ns, all);
         at += all;
+        float x[EV_PER];  // (all on their way before the first is stored)
+        if (WO) {
 #pragma unroll
-        for (uint32_t u = 0; u < EV_PER; u++) {
+            for (uint32_t u = 0; u < EV_PER; u++) x[u] = w[stays >> u & 1 ? b + mine + u * 64 : 0];
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < EV_PER; u++)
             if (u < per) {
-                const uint32_t i = b + mine + u * 64;
                 const bool stay = stays >> u & 1;
                 const uint64_t who = __ballot(stay);
                 if (stay) {
                     const uint32_t r = to + below(who);
-                    list[r] = (int32_t)i;
-                    if (WO) WO[sh * wost + r] = w[i];
+                    list[r] = (int32_t)(b + mine + u * 64);
+                    if (WO) WO[sh * wost + r] = x[u];
                 }
                 to += __popcll(who);
             }
-        }
     }
 }
 

@@ -468,6 +468,29 @@ def test_read(enc, t, D, heads, lens, rows):
     assert np.array_equal(host(only), host(v))
 
 
+@gpu
+def test_append_and_read_many_sequences(enc):
+    """More sequences than a wavefront has lanes, some with no new token."""
+    rng = np.random.default_rng(23)
+    new = [int(x) for x in rng.integers(0, 4, 150)]
+    new[149] = 70
+    lens = [int(x) + m for x, m in zip(rng.integers(0, 130, 150), new)]
+    d = Dev(lens, 1, 16, 24)
+    st = starts(new)
+    k, v = (rng.standard_normal((st[-1], 1, 16)).astype(np.float32) for _ in range(2))
+    enc.kv_append(d.cache, d.seqs, dev(k), dev(v), ints(st), st[-1])
+    ko, vo = (torch.empty(st[-1], 1, 16, device="cuda") for _ in range(2))
+    enc.kv_read(d.cache, d.seqs, ko, vo, ints(st), st[-1])
+    enc.sync()
+    for s, n in enumerate(lens):
+        d.c.append(d.table[s], n, k[st[s]:st[s + 1]], v[st[s]:st[s + 1]])
+    d.same()
+    same_codes(d)
+    for s, n in enumerate(lens):
+        for got, ref in zip((ko, vo), d.c.values(d.table[s], n)):
+            assert np.array_equal(host(got)[st[s]:st[s + 1]], ref[n - new[s]:].astype(np.float32).astype(np.float64))
+
+
 def decode_ref(d, q, window, scale):
     """Outputs [B][T][H][D] and weights [B][KV][tokens] of the oracle."""
     Bn, T, H, D = q.shape
@@ -660,6 +683,31 @@ def test_evict(enc, D, heads, lens, keep, sink, recent):
                 p, e = to[s, b], min(64, m - 64 * b)
                 assert gks[p, h] == tk[b] and gvs[p, h] == tv[b]
                 assert np.array_equal(gk[p, h, :e], ck[64 * b:64 * b + e]) and np.array_equal(gv[p, h, :e], cv[64 * b:64 * b + e])
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["steps", "equal", "nan", "some nan", "tiny"])
+@pytest.mark.parametrize("keep,sink,recent", [(700, 3, 64), (64, 64, 0), (1000, 0, 0)])
+def test_evict_selects(enc, kind, keep, sink, recent):
+    """Which tokens stay, of up to 33000: steps, equal weights, NaN (all, and more than may go), denormals."""
+    lens = [33000, 16385, 16384, 1001, 1000]
+    d = Dev(lens, 1, 16, keep, spare=16)
+    n = d.stride * 64
+    w = {"steps": d.rng.integers(0, 300, (5, 1, n)) / 8, "equal": np.full((5, 1, n), 0.25), "nan": np.full((5, 1, n), np.nan),
+         "some nan": np.where(d.rng.random((5, 1, n)) < 0.99, np.nan, d.rng.random((5, 1, n))),
+         "tiny": d.rng.integers(-5, 9, (5, 1, n)) * 1e-45}[kind].astype(np.float32)
+    nb = (keep + 63) // 64
+    dto, new_len = torch.full((5, nb), -1, dtype=torch.int32, device="cuda"), ints([0] * 5)   # (no pages: the list is what counts)
+    kept, wo = torch.full((5, 1, keep), -9, dtype=torch.int32, device="cuda"), torch.full((5, 1, keep), 7.0, device="cuda")
+    enc.kv_evict(d.cache, d.seqs, d.cache, ok.KVSeqs(dto, new_len, 5, nb), keep, sink, recent, dev(w), n, wo, keep, kept)
+    enc.sync()
+    for s, m in enumerate(lens):
+        x = np.nan_to_num(w[s, 0, :m].astype(np.float64), nan=-np.inf)
+        inner = sorted(range(sink, m - recent), key=lambda i: (-x[i], i))[:keep - sink - recent] if m > keep else []
+        want = sorted([*range(sink), *inner, *range(m - recent, m)]) if m > keep else list(range(m))
+        assert host(kept)[s, 0].tolist() == want + [-1] * (keep - len(want)), (s, m)
+        assert np.array_equal(host(wo)[s, 0, :len(want)], w[s, 0, want].astype(np.float64), equal_nan=True)
+        assert host(new_len)[s] == min(m, keep)
 
 
 @gpu
