@@ -21,12 +21,12 @@
 // weights: six of the nine products of parts, the others are below 2^-22 of the
 // whole.
 //
-// Measured (MI355X): f16, 8192 rows x 40 heads of 128 709-730 us, 960 TFLOP/s; a matrix
+// Measured (MI355X): f16, 8192 rows x 40 heads of 128 700-740 us, 930-980 TFLOP/s; a matrix
 // product of 8192 in f16 runs at 1119 there, both at the 2.0 GHz or less that the card's
-// power leaves.  Without its loads from memory the kernel took 14 % less, without the
-// reads of LDS 11 %: no one of matrix cores (half their time), vector units and LDS bounds
-// it alone.  8 packed bf16 prompts of up to 1111 x 16 heads 38.6 us, where the first
-// order of tiles (the last sequence's first) took 47.
+// power leaves.  Without its loads from memory the variant named at the pass took 14 %
+// less, without its reads of LDS 11 %: no one of matrix cores (57 % of their time), vector
+// units (50 %) and LDS bounds it alone.  8 packed bf16 prompts of up to 1111 x 16 heads 37 us; with the last
+// sequence's tiles first 47.
 #pragma once
 #include <type_traits>
 
@@ -116,11 +116,6 @@ template <class E>
 __device__ __forceinline__ float at_half(uint32_t x) {
     if constexpr (__is_same(E, _Float16)) return (float)__builtin_bit_cast(_Float16, (uint16_t)x);
     else return __uint_as_float(x << 16);
-}
-
-__device__ __forceinline__ float at_max3(float x, float y, float z) {
-    asm("v_max3_f32 %0, %0, %1, %2" : "+v"(x) : "v"(y), "v"(z));
-    return x;
 }
 
 // the larger of x here and in lane ^ 32
@@ -371,7 +366,7 @@ __global__ __launch_bounds__(S::NT, S::WAVES) void attn_prompt_kernel(AttnArgs a
 #pragma unroll
         for (int t = 0; t < TT; t++)
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) x = at_max3(x, s[t][i], s[t][i + 1]);
+            for (int i = 0; i < 16; i++) x = fmaxf(x, s[t][i]);
         x = at_max32(x);
         if (__ballot(x > limit)) {
             const float nm = fmaxf(m, x);
