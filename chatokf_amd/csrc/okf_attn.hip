@@ -76,20 +76,28 @@ int check_rows(const okf_kv_cache *c, const okf_kv_seqs *s, const void *k, const
     return OKF_OK;
 }
 
-// The splits of okf_attn_decode: how many page ranges each sequence and kv head
-// is cut into, so that the workgroups fill the CUs (as many at a time on each as the
-// kernel's registers leave room for: two for up to 128 dimensions, one past that), but no range of less than a page for each of a
-// workgroup's wavefronts; batches of ragged sequences get twice that, so that the
-// short ones' workgroups make room for the long ones'.  The partial results go to
-// the context's buffer; where it may not grow, as many splits as it holds.
+// The splits of okf_attn_decode: how many page ranges each sequence and kv head is cut
+// into.  So many that the workgroups fill the CUs (as many at a time on each as the kernel's
+// registers leave room for: two for up to 128 dimensions, one past that), but with a page
+// for each of a workgroup's wavefronts, and two where that would be more workgroups than CUs
+// (one sequence of 40000 tokens x 2 kv heads: 15.5 us, with one page 17.6; 1999 tokens x 8, 64
+// workgroups: 12.3, with one page 10.8).  Batches of ragged sequences get up to twice that, so
+// that the short ones' workgroups make room for the long ones', where four pages are left for
+// each wavefront (32 of up to 8192 tokens 69 us, without 75; 20 of up to 3000 x 8 kv heads of
+// 96 with weights 29, without 26).  The partial results go to the context's buffer; where it
+// may not grow, as many splits as it holds.
 constexpr uint64_t DEC_KEPT = 256ull << 20;  // bytes of scores at most
 int plan_decode(okf_ctx *c, DecArgs &a) {
     const uint64_t rows = (uint64_t)a.tokens * (a.heads / a.c.heads), rpb = rows > 16 ? 32 : 16;
     a.rb = (uint32_t)((rows + rpb - 1) / rpb);
     const uint64_t base = (uint64_t)a.s.count * a.c.heads * a.rb;
-    uint64_t want = (uint64_t)c->cus * (a.c.dim <= 128 ? 2 : 1) * (a.s.count > 1 ? 2 : 1);
     const uint64_t span = a.window ? std::min<uint64_t>(((uint64_t)a.window + a.tokens) / KV_B + 2, a.s.stride) : a.s.stride;
-    uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>({(want + base - 1) / base, (span + DEC_W - 1) / DEC_W, DEC_SPLITS}));
+    auto up = [](uint64_t x, uint64_t y) { return (x + y - 1) / y; };
+    const uint64_t want = (uint64_t)c->cus * (a.c.dim <= 128 ? 2 : 1);
+    const uint64_t each = base * up(span, DEC_W) <= c->cus ? 1 : 2;
+    uint64_t splits = std::min(up(want, base), up(span, each * DEC_W));
+    if (a.s.count > 1) splits = std::max(splits, std::min(up(2 * want, base), up(span, 4 * DEC_W)));
+    splits = std::min<uint64_t>(splits, DEC_SPLITS);
     auto bytes = [&](uint64_t n) {  // m and l, then partial outputs
         return base * n * rpb * 2 * sizeof(float) + (n > 1 ? base * n * rpb * a.c.dim * sizeof(float) : 0);
     };
