@@ -155,7 +155,8 @@ int okf_attn_prompt(okf_ctx *c, const okf_attn *p) {
     if (!p || !p->q || !p->k || !p->v || !p->o || !p->q_start || !p->k_start) return OKF_E_ARG;
     if (!attn_type(p->type)) return OKF_E_TYPE;
     if (!p->heads || !p->kv_heads || p->heads % p->kv_heads || p->heads > 65535 || !good_dim(p->dim)) return OKF_E_SHAPE;
-    if (!p->seqs || !p->n_q || !p->n_k || p->n_q > 0x7FFFFFFFu || p->n_k > 0x7FFFFFFFu) return OKF_E_SHAPE;
+    // (rows are counted in 32 bits with a sign, up to a workgroup's past the last)
+    if (!p->seqs || !p->n_q || !p->n_k || p->n_q > 0x7FFFFF00u || p->n_k > 0x7FFFFF00u) return OKF_E_SHAPE;
     const uint32_t size = p->type == F32 ? 4 : 2;
     AttnArgs a{p->q, p->k, p->v, p->o, p->heads, p->kv_heads, p->dim, p->seqs, p->n_q, p->n_k, p->q_start, p->k_start,
                p->q_stride, p->k_stride, p->v_stride, p->o_stride, p->q_head, p->k_head, p->v_head, p->o_head,

@@ -264,7 +264,7 @@ typedef struct {
     void *o;                        /* n_q rows of heads x dim */
     int32_t type;                   /* of q, k, v and o: OKF_TYPE_F32, _F16 or _BF16 */
     uint32_t heads, kv_heads, dim;
-    uint32_t seqs, n_q, n_k;        /* sequences, query rows, key rows in all */
+    uint32_t seqs, n_q, n_k;        /* sequences, query rows, key rows in all (rows: 2^31 - 256 at most) */
     const int32_t *q_start, *k_start;   /* device memory, seqs + 1 each */
     uint64_t q_stride, k_stride, v_stride, o_stride; /* values from a row to the next (0: dense) */
     uint64_t q_head, k_head, v_head, o_head;         /* values from a head to the next (0: dim) */

@@ -1,0 +1,36 @@
+"""Attention at the ends of its arguments' ranges: windows as large as the type, scales and
+queries of any finite size.  Bounds as in test_attn.py; scaling by a power of two is exact, so
+that an input scaled one way and its scale the other leave the bound as it was."""
+import numpy as np
+import pytest
+
+import attn_oracle as ao
+
+torch = pytest.importorskip("torch")
+import chatokf_amd as ok  # noqa: E402
+from test_attn import TYPES, attn, dev, fails, gpu, host, run_prompt, starts, tol  # noqa: E402
+
+
+@gpu
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("window", [0xFFFFFFFF, 0x80000000, 0x7FFFFFFF, 0x7FFFFFFE, 0x7FFFFFC0, 200, 25])
+@pytest.mark.parametrize("H,KV,D,qlens,klens", [(2, 1, 128, [100, 20, 70], [30, 0, 70]),   # positions from -70 on
+                                                (40, 2, 64, [700, 330], [200, 301])])     # 128 rows a workgroup
+def test_prompt_window_larger_than_the_keys(enc, t, window, H, KV, D, qlens, klens):
+    """More queries than keys: the first tile's positions are below zero, whatever the window."""
+    rng = np.random.default_rng(D + len(qlens))
+    qs, ks = starts(qlens), starts(klens)
+    q, k, v = (dev(rng.standard_normal((s[-1], h, D)).astype(np.float32), TYPES[t]) for s, h in ((qs, H), (ks, KV), (ks, KV)))
+    got = run_prompt(enc, q, k, v, qs, ks, t, window, D ** -0.5, H, KV, D)
+    q, k, v = host(q), host(k), host(v)
+    ref = ao.prompt(q, k, v, qs, ks, window, D ** -0.5)
+    assert np.abs(got - ref).max() <= tol(q, k, v, D ** -0.5, max(klens), D, t)
+
+
+@pytest.mark.parametrize("over,status", [({"n_q": 0x7FFFFF00}, ok.OKF_E_NODEV), ({"n_q": 0x7FFFFF01}, ok.OKF_E_SHAPE),
+                                         ({"n_k": 0x7FFFFF00}, ok.OKF_E_NODEV), ({"n_k": 0x7FFFFF01}, ok.OKF_E_SHAPE)])
+def test_prompt_rows_that_32_bits_hold(over, status):
+    """A tile's rows and keys are numbered past the last one."""
+    e = ok.Enc(-1)
+    fails(lambda: attn(e, **over), status)
+    e.close()
