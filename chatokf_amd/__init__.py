@@ -393,7 +393,8 @@ class Enc:
 
     def kv_evict(self, src: KVCache, seqs: KVSeqs, dst: KVCache, to: KVSeqs, keep: int, sink: int, recent: int, w_in,
                  w_in_stride: int, w_out, w_out_stride: int, kept):
-        """okf_kv_evict: cut each sequence to `keep` tokens a head, by accumulated attention weight."""
+        """okf_kv_evict: cut each sequence to `keep` tokens a head, by accumulated attention weight.
+        Lengths (to.lens = seqs.lens) and weights (w_out = w_in, one stride) may be written in place."""
         self._check(self._lib.okf_kv_evict(self.h, ctypes.byref(src.c()), ctypes.byref(seqs.c()),
                                            ctypes.byref(dst.c()), ctypes.byref(to.c()), keep, sink, recent,
                                            _ptr(w_in), w_in_stride, _ptr(w_out), w_out_stride, _ptr(kept)),

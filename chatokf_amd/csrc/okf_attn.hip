@@ -57,6 +57,18 @@ bool row_stride(uint64_t &st, uint64_t least, uint32_t size) {
     return st >= least && st <= (1ull << 40) && st * size % 16 == 0;
 }
 
+// Whether n rows of la values, sa apart, share memory with n rows of lb values, sb apart.
+bool rows_meet(const float *a, uint64_t sa, uint64_t la, const float *b, uint64_t sb, uint64_t lb, uint64_t n) {
+    const uint64_t pa = (uint64_t)(uintptr_t)a / sizeof(float), pb = (uint64_t)(uintptr_t)b / sizeof(float);
+    if (pa + (n - 1) * sa + la <= pb || pb + (n - 1) * sb + lb <= pa) return false;
+    for (uint64_t i = 0, j = 0; i < n && j < n;) {
+        if (pa + i * sa + la <= pb + j * sb) i++;
+        else if (pb + j * sb + lb <= pa + i * sa) j++;
+        else return true;
+    }
+    return false;
+}
+
 // Arguments that okf_kv_append and okf_kv_read share, and their grid: n rows of
 // `count` sequences touch at most n / 64 + 2 count page blocks.
 int check_rows(const okf_kv_cache *c, const okf_kv_seqs *s, const void *k, const void *v, int32_t type,
@@ -256,8 +268,14 @@ int okf_kv_evict(okf_ctx *c, const okf_kv_cache *src, const okf_kv_seqs *from, c
     const uint32_t group = std::min(from->count, 65535 / src->heads);
     const uint32_t groups = (from->count + group - 1) / group;
     if (groups > 65535) return OKF_E_SHAPE;
+    // lengths and weights may be written in place (both kernels say why), not beside their places
+    const uint64_t apart = from->len > to->len ? from->len - to->len : to->len - from->len;
+    if (apart && apart < from->count) return OKF_E_ARG;
+    if (w_out && !(w_out == w_in && w_out_stride == w_in_stride) &&
+        rows_meet(w_in, w_in_stride, (uint64_t)from->stride * KV_B, w_out, w_out_stride, keep, rows))
+        return OKF_E_ARG;
     if ((st = begin(c))) return st;
-    hipLaunchKernelGGL(kv_select_kernel, dim3((uint32_t)rows), dim3(EV_NT), 0, c->stream, seqs_of(from), to->len,
+    hipLaunchKernelGGL(kv_select_kernel, dim3((uint32_t)rows), dim3(EV_NT), 0, c->stream, seqs_of(from),
                        src->heads, keep, sink, recent, w_in, w_in_stride, w_out, w_out_stride, kept);
     const dim3 grid((keep + KV_B - 1) / KV_B, group * src->heads, groups);
     with_dims(src->dim, [&](auto nd) {

@@ -356,6 +356,11 @@ __global__ __launch_bounds__(KV_NT) void kv_read_kernel(KvCache c, KvSeqs q, T *
     }
 }
 
+// The tokens that sequence s of an eviction holds in its table.
+__device__ __forceinline__ uint32_t kv_held(const KvSeqs &q, uint64_t s) {
+    return min((uint32_t)max(q.len[s], 0), (uint32_t)min((uint64_t)q.stride * KV_B, (uint64_t)0x7FFFFFFF));
+}
+
 // A weight as an unsigned key of the same order (-0 as 0, NaN lowest).
 __device__ __forceinline__ uint32_t kv_key(float w) {
     if (w != w) return 0;
@@ -385,20 +390,20 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *red, uint32
 // of the last token that stays (a count by the top 11 bits, then by the next 11 and the
 // last 10) and lists the kept tokens in order.  A wavefront takes 1024 tokens side by
 // side, 64 at a time, so that a token's place among its wavefront's is a count of lanes;
-// up to EV_ALL tokens' keys stay in registers from count to count.
+// up to EV_ALL tokens' keys stay in registers from count to count.  The weights may be W's own
+// rows: a kept one goes to its own place or to a lower one, which no later round reads, and
+// those of one round are all read before the first of them is written.
 constexpr int EV_NT = 1024;
 constexpr uint32_t EV_PER = 16, EV_ALL = EV_NT * EV_PER;
-__global__ __launch_bounds__(EV_NT) void kv_select_kernel(KvSeqs from, int32_t *__restrict__ new_len, uint32_t heads,
-                                                          uint32_t keep, uint32_t sink, uint32_t recent,
-                                                          const float *__restrict__ W, uint64_t wst, float *WO,
+__global__ __launch_bounds__(EV_NT) void kv_select_kernel(KvSeqs from, uint32_t heads, uint32_t keep, uint32_t sink,
+                                                          uint32_t recent, const float *W, uint64_t wst, float *WO,
                                                           uint64_t wost, int32_t *__restrict__ kept) {
     __shared__ uint32_t hist[2048], red[EV_NT / 64], pick[2];
     const uint32_t tid = threadIdx.x, s = blockIdx.x / heads, h = blockIdx.x % heads, lane = tid & 63;
     const uint64_t sh = (uint64_t)s * heads + h;
-    const uint32_t len = min((uint32_t)max(from.len[s], 0), (uint32_t)min((uint64_t)from.stride * KV_B, (uint64_t)0x7FFFFFFF));
+    const uint32_t len = kv_held(from, s);
     const float *w = W + sh * wst;
     int32_t *list = kept + sh * keep;
-    if (h == 0 && tid == 0) new_len[s] = (int32_t)min(len, keep);
     if (len <= keep) {
         for (uint32_t i = tid; i < keep; i += EV_NT) {
             list[i] = i < len ? (int32_t)i : -1;
@@ -502,10 +507,11 @@ __global__ __launch_bounds__(EV_NT) void kv_select_kernel(KvSeqs from, int32_t *
             }
         uint32_t to = at + share(ns, all);
         at += all;
-        float x[EV_PER];  // (all on their way before the first is stored)
+        float x[EV_PER];
         if (WO) {
 #pragma unroll
             for (uint32_t u = 0; u < EV_PER; u++) x[u] = w[stays >> u & 1 ? b + mine + u * 64 : 0];
+            __syncthreads();  // (the other wavefronts' too, before the first is written: WO may be W)
         }
 #pragma unroll
         for (uint32_t u = 0; u < EV_PER; u++)
@@ -523,7 +529,8 @@ __global__ __launch_bounds__(EV_NT) void kv_select_kernel(KvSeqs from, int32_t *
 }
 
 // okf_kv_evict, second launch: workgroup (new block, head, sequence) gathers
-// the listed tokens and rounds them to the block's scale.  Keys are rows; a value is a
+// the listed tokens and rounds them to the block's scale.  The new lengths are written
+// here, where no workgroup reads a length but the one that writes it: they may be the old ones' array.  Keys are rows; a value is a
 // byte in each of a page's rows.  Wavefront g takes the tokens of byte group g (kv_slot)
 // of every source page: a lane loads the group's 16 bytes of its rows, which is all of
 // the page's lines that hold kept tokens, and puts each kept byte to its new place in
@@ -540,6 +547,8 @@ __global__ __launch_bounds__(KV_NT) void kv_gather_kernel(KvCache c, KvSeqs from
     const uint32_t blk = blockIdx.x, h = blockIdx.y % c.heads, tid = threadIdx.x;
     const uint64_t s = (uint64_t)blockIdx.z * (gridDim.y / c.heads) + blockIdx.y / c.heads;
     if (s >= from.count) return;
+    // (by the last wavefront: the first one has loads enough to wait for)
+    if (blk == 0 && h == 0 && tid == KV_NT - 1) to.len[s] = (int32_t)min(kv_held(from, s), keep);
     const int32_t *list = kept + (s * c.heads + h) * keep + blk * KV_B;
     const uint32_t left = min(keep - blk * KV_B, KV_B), D = c.dim;
     const int32_t page = to.pages[s * to.stride + blk];

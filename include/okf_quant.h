@@ -343,10 +343,12 @@ int okf_attn_decode(okf_ctx *ctx, const okf_kv_cache *cache, const okf_kv_seqs *
  * (ties to the lower index; NaN lowest), in their order; a sequence of at most
  * `keep` tokens stays whole.  The tokens go to the pages of `to`, which must
  * be other ones than `from`'s (they may be of the same cache); to->len is
- * written.  A new page's scale is the largest of its tokens' scales; codes
- * under another scale are rounded (64-bit product with the scales' quotient).
- * kept[s][head][keep]: the tokens' old indices, then -1.  w_out, if not NULL:
- * their weights, in w_out[s][head][0 .. to->len).  sink + recent <= keep <=
+ * written, and may be from->len.  A new page's scale is the largest of its
+ * tokens' scales; codes under another scale are rounded (64-bit product with
+ * the scales' quotient).  kept[s][head][keep]: the tokens' old indices, then
+ * -1.  w_out, if not NULL: their weights, in w_out[s][head][0 .. to->len);
+ * w_out = w_in with the same stride writes them in place.  Lengths or weights
+ * that overlap in any other way are an OKF_E_ARG.  sink + recent <= keep <=
  * 64 to->stride; w rows as for okf_attn_decode. */
 int okf_kv_evict(okf_ctx *ctx, const okf_kv_cache *src, const okf_kv_seqs *from, const okf_kv_cache *dst,
                  const okf_kv_seqs *to, uint32_t keep, uint32_t sink, uint32_t recent, const float *w_in,
