@@ -35,7 +35,7 @@ namespace okf {
 
 constexpr uint32_t DEC_NT = 256, DEC_W = DEC_NT / 64;
 constexpr float DEC_P = 8355711.0f;      // 0x7F7F7F: the largest 3-digit number with signed byte digits
-constexpr float LOG2E = 1.4426950408889634f;
+constexpr double LOG2E = 1.4426950408889634;
 
 struct DecArgs {
     KvCache c;
@@ -66,7 +66,8 @@ __device__ __forceinline__ void dec_digits(uint32_t a, uint32_t b, uint32_t c, u
 template <int KS, int NR>
 struct DecQuery {
     int32x4 d[NR][3][KS];
-    float f[NR];                // score of one unit of Q code, times log2 e
+    float f[NR];                // f 2^fe: score of one unit of Q code, times log2 e (without a
+    int fe[NR];                 // page's scale it may leave the range of fp32)
     uint32_t hi[NR], lo[NR];
     uint32_t hi_min, hi_max, lo_min, lo_max;   // over the workgroup's rows
 
@@ -106,18 +107,20 @@ struct DecQuery {
             m = fmaxf(m, __shfl_xor(m, 32));
             bad += __shfl_xor(bad, 16);
             bad += __shfl_xor(bad, 32);
-            // m = c 2^e, c < 1: 2^(23 - e) where c 2^23 fits three digits
+            // m = c 2^e, c < 1: units of 2^(e - 23) where c 2^23 fits three digits (by exponents: no
+            // fp32 number is the unit's inverse for every m)
             int e = __builtin_amdgcn_frexp_expf(m);
-            e = max(min(e + (__builtin_amdgcn_ldexpf(m, 23 - e) > DEC_P), 127), -100);
-            const float up = __builtin_amdgcn_ldexpf(1.0f, 23 - e);
-            f[n] = (__builtin_amdgcn_ldexpf(a.scale, e - 23) + bad) * LOG2E;
+            e += __builtin_amdgcn_ldexpf(m, 23 - e) > DEC_P;
+            const double c = (double)a.scale * LOG2E;
+            f[n] = (float)__builtin_amdgcn_frexp_mant(c) + bad;
+            fe[n] = __builtin_amdgcn_frexp_exp(c) + e - 23;
 #pragma unroll
             for (int k = 0; k < KS; k++) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     uint32_t y[4];
 #pragma unroll
-                    for (int j = 0; j < 4; j++) y[j] = (uint32_t)(__float2int_rn(x[k][i][j] * up) + 0x808080);
+                    for (int j = 0; j < 4; j++) y[j] = (uint32_t)(__float2int_rn(__builtin_amdgcn_ldexpf(x[k][i][j], 23 - e)) + 0x808080);
                     int p0, p1, p2;
                     dec_digits(y[0], y[1], y[2], y[3], p0, p1, p2);
                     d[n][0][k][i] = p0;
@@ -152,7 +155,7 @@ __device__ __forceinline__ void dec_scores(float (&s)[NR][16], const int32x4 (&k
     const bool whole = j0 + KV_B <= q.hi_min && j0 >= q.lo_max;
 #pragma unroll
     for (int n = 0; n < NR; n++) {
-        const float f = q.f[n] * ks;
+        const float f = __builtin_amdgcn_ldexpf(q.f[n] * ks, q.fe[n]);
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             int32x4 c0 = {0, 0, 0, 0}, c1 = c0, c2 = c0;

@@ -8,7 +8,7 @@ import attn_oracle as ao
 
 torch = pytest.importorskip("torch")
 import chatokf_amd as ok  # noqa: E402
-from test_attn import TYPES, attn, dev, fails, gpu, host, run_prompt, starts, tol  # noqa: E402
+from test_attn import TYPES, Dev, attn, decode_ref, dev, fails, gpu, host, run_prompt, starts, tol  # noqa: E402
 
 
 @gpu
@@ -34,3 +34,25 @@ def test_prompt_rows_that_32_bits_hold(over, status):
     e = ok.Enc(-1)
     fails(lambda: attn(e, **over), status)
     e.close()
+
+
+@gpu
+@pytest.mark.parametrize("H", [8, 40])     # (with weights from the scores that are kept, and made again)
+@pytest.mark.parametrize("qe,se,ke", [(127, -127, 0), (126, -126, 0), (-126, 126, 0), (-140, 120, 20), (0, -120, 120),
+                                      (0, 100, -100), (100, 0, -100)])
+def test_decode_sizes(enc, H, qe, se, ke):
+    """Queries, scale and key scales 2^qe, 2^se and 2^ke of the usual: from the largest numbers to denormal ones."""
+    d = Dev([333, 70], 1, 64, 15)
+    d.c.ks[:] = np.ldexp(d.c.ks, ke)
+    d.push()
+    q = d.rng.standard_normal((2, 1, H, 64)).astype(np.float32)
+    q = np.ldexp(np.float32(1.99) * q / np.abs(q).max(-1, keepdims=True), qe)
+    assert np.isfinite(q).all()
+    scale = 2.0 ** (se - 3)
+    o, wo = torch.empty(q.shape, device="cuda"), torch.zeros((2, 1, d.stride * 64), device="cuda")
+    enc.attn_decode(d.cache, d.seqs, dev(q), o, 1, H, scale, w_out=wo, w_stride=d.stride * 64)
+    enc.sync()
+    ref, add = decode_ref(d, q, 0, scale)
+    bound = tol(np.ldexp(q.astype(np.float64), -qe), np.full((1, 64), 5.2), np.full(1, 5.2), 0.125, 333, 64)
+    assert np.abs(host(o) - ref).max() <= bound
+    assert np.abs(host(wo) - add).max() <= bound / 5.2 * H + 4 * 2.0 ** -24 * H
