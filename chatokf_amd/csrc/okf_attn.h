@@ -198,7 +198,7 @@ __global__ __launch_bounds__(S::NT, S::WAVES) void attn_prompt_kernel(AttnArgs a
     const uint2 rq = kv_rows(a.q_start, it.seq, a.nq), rk = kv_rows(a.k_start, it.seq, a.nk);
     // (a window of all keys is none; a smaller one taken from a position, which is below zero where
     // there are more queries than keys, is above -nq and so within 32 bits)
-    const int nq = rq.y - rq.x, nk = rk.y - rk.x, i0 = it.at * BM, w = a.window < (uint32_t)nk ? (int)a.window : 0;
+    const int nq = rq.y - rq.x, nk = rk.y - rk.x, i0 = it.at * BM, w = a.window && a.window < (uint32_t)nk ? (int)a.window : 0;
     const int kh = head / (a.heads / a.kv_heads);
     // positions: of the workgroup's first and last row, the wavefront's, the lane's
     const int p_first = nk - nq + i0, p_last = nk - nq + min(i0 + BM, nq) - 1;
