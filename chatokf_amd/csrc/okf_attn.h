@@ -210,7 +210,9 @@ __global__ __launch_bounds__(S::NT, S::WAVES) void attn_prompt_kernel(AttnArgs a
     // queries: parts of dimensions 16 k + 8 h .. + 7 of the lane's row.  The scale's sign goes to them.
     float c = a.scale * 1.4426950408889634f;
     const uint32_t flip = c < 0 ? 0x80008000u : 0;
-    c = fabsf(c) < 1e-30f ? 1e-30f : fabsf(c);  // (a factor of 0 would make NaN of a masked -inf)
+    // (a factor of 0 would make NaN of a masked -inf; the smallest number there is takes any two
+    // scores less than 2^-19 apart)
+    c = c == 0 ? 0x1p-149f : fabsf(c);
     u32x4v q[NP][KS];
     const T *qrow = (const T *)a.q + (uint64_t)(rq.x + min(row, nq - 1)) * a.qs + (uint64_t)head * a.qh;
 #pragma unroll

@@ -27,6 +27,21 @@ def test_prompt_window_larger_than_the_keys(enc, t, window, H, KV, D, qlens, kle
     assert np.abs(got - ref).max() <= tol(q, k, v, D ** -0.5, max(klens), D, t)
 
 
+@gpu
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_prompt_scale_of_any_size(enc, t):
+    """Large inputs under a scale as small: a power of two more here and less there changes nothing;
+    a scale of 0 weighs all keys alike, whatever the products."""
+    rng = np.random.default_rng(17)
+    n, H, KV, D = 150, 2, 1, 64
+    q, k, v = (rng.standard_normal((n, h, D)).astype(np.float32) for h in (H, KV, KV))
+    for e, scale in ((56, 2.0 ** -115), (60, 0.0), (-40, 2.0 ** 77)):
+        q_, k_, v_ = dev(np.ldexp(q, e), TYPES[t]), dev(np.ldexp(k, e), TYPES[t]), dev(v, TYPES[t])
+        got = run_prompt(enc, q_, k_, v_, [0, n], [0, n], t, 0, scale, H, KV, D)
+        ref = ao.prompt(host(q_), host(k_), host(v_), [0, n], [0, n], 0, scale)
+        assert np.abs(got - ref).max() <= tol(q, k, v, scale * 4.0 ** e, n, D, t), e
+
+
 @pytest.mark.parametrize("over,status", [({"n_q": 0x7FFFFF00}, ok.OKF_E_NODEV), ({"n_q": 0x7FFFFF01}, ok.OKF_E_SHAPE),
                                          ({"n_k": 0x7FFFFF00}, ok.OKF_E_NODEV), ({"n_k": 0x7FFFFF01}, ok.OKF_E_SHAPE)])
 def test_prompt_rows_that_32_bits_hold(over, status):
