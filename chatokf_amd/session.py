@@ -58,11 +58,11 @@ class Chat:
         return torch.tensor([0, n], dtype=torch.int32, device="cuda")
 
     def _append(self, k, v):
-        n = k.shape[0]
+        n, cut = k.shape[0], min(self.n, self.keep)
+        if cut + n > self.limit:  # (refused before anything is evicted for it)
+            raise ValueError(f"{n} new tokens do not fit beside {cut} of {self.limit}")
         if self.n + n > self.limit:
             self.evict()
-        if self.n + n > self.limit:
-            raise ValueError(f"{n} new tokens do not fit beside {self.n} of {self.limit}")
         self.n += n
         self.lens[self.at].fill_(self.n)
         self.layer.enc.kv_append(self.cache, self.seqs[self.at], k, v, self._starts(n), n)
