@@ -29,7 +29,7 @@ EXPORTS = (
     "okf_ctx_create", "okf_ctx_destroy", "okf_ctx_stream", "okf_ctx_reserve", "okf_row_bytes",
     "okf_gemv", "okf_gemv_silu", "okf_gemv_gate_up", "okf_ffn", "okf_silu_mul", "okf_gemm", "okf_gemm_tile", "okf_dequant_row",
     "okf_embed_batch", "okf_add_rmsnorm_batch", "okf_argmax_rows", "okf_argmax_rows_noalloc",
-    "okf_stream_read", "okf_attn_prompt", "okf_attn_decode", "okf_kv_append", "okf_kv_read", "okf_kv_evict",
+    "okf_stream_read", "okf_attn_prompt", "okf_attn_decode", "okf_attn_reserve", "okf_kv_append", "okf_kv_read", "okf_kv_evict",
     "okf_parallel_begin",
     "okf_parallel_end", "okf_sync", "okf_set_fault_rate", "okf_last_hip_error", "okf_strerror",
     "okf_gguf_open", "okf_gguf_close", "okf_gguf_tensor_count", "okf_gguf_tensor_at", "okf_gguf_find",
@@ -125,6 +125,7 @@ def _lib():
             "okf_stream_read": [vp, vp, ctypes.c_uint64, vp],
             "okf_attn_prompt": [vp, ctypes.POINTER(OkfAttn)],
             "okf_attn_decode": [vp, KC, KS, vp, vp, u32, u32, ctypes.c_float, u32, vp, vp, u64],
+            "okf_attn_reserve": [vp, u32, u32, u32, u32, u32, u32, i32],
             "okf_kv_append": [vp, KC, KS, vp, vp, i32, vp, u32, u64, u64],
             "okf_kv_read": [vp, KC, KS, vp, vp, i32, vp, u32, u64, u64],
             "okf_kv_evict": [vp, KC, KS, KC, KS, u32, u32, u32, vp, u64, vp, u64, vp],
@@ -378,6 +379,12 @@ class Enc:
         self._check(self._lib.okf_attn_decode(self.h, ctypes.byref(cache.c()), ctypes.byref(seqs.c()), _ptr(q),
                                               _ptr(out), tokens, heads, scale, window, _ptr(w_in), _ptr(w_out),
                                               w_stride), "okf_attn_decode")
+
+    def attn_reserve(self, seqs: int, stride: int, heads: int, kv_heads: int, dim: int, tokens: int = 1,
+                     weights: bool = False):
+        """okf_attn_reserve: allocate the scratch of attn_decode calls of up to these sizes now."""
+        self._check(self._lib.okf_attn_reserve(self.h, seqs, stride, heads, kv_heads, dim, tokens, int(weights)),
+                    "okf_attn_reserve")
 
     def kv_append(self, cache: KVCache, seqs: KVSeqs, k, v, start, n: int, type: int = F32, k_stride: int = 0,
                   v_stride: int = 0):

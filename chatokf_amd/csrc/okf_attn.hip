@@ -99,25 +99,38 @@ int check_rows(const okf_kv_cache *c, const okf_kv_seqs *s, const void *k, const
 // 96 with weights 29, without 26).  The partial results go to the context's buffer; where it
 // may not grow, as many splits as it holds.
 constexpr uint64_t DEC_KEPT = 256ull << 20;  // bytes of scores at most
+uint64_t up(uint64_t x, uint64_t y) { return (x + y - 1) / y; }
+
+// The query rows of a kv head in blocks of 16 or 32, all sequences' and kv heads' blocks, and the
+// workgroups that fill the CUs.
+struct DecRows {
+    uint64_t rows, rpb, rb, base, want;
+    DecRows(const okf_ctx *c, uint64_t seqs, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t tokens)
+        : rows((uint64_t)tokens * (heads / kv_heads)), rpb(rows > 16 ? 32 : 16), rb(up(rows, rpb)), base(seqs * kv_heads * rb),
+          want((uint64_t)c->cus * (dim <= 128 ? 2 : 1)) {}
+    // bytes of scratch for n workgroups: maxima and sums, and the partial outputs of several splits
+    uint64_t bytes(uint64_t n, uint32_t dim, bool several) const { return n * rpb * (2 + (several ? dim : 0)) * sizeof(float); }
+};
+
+// Bytes of the scores that are kept for the weights of up to `rows` query rows of a kv head, 0 where
+// that is not less to write and read than the keys are to read again (8 sequences of up to 16000
+// tokens, 2 rows of 64: 31.6 us without); more than DEC_KEPT are not kept.
+uint64_t dec_kept(uint64_t heads, uint64_t rows, uint32_t dim, uint64_t stride) {
+    if (rows > 16 || 8 * rows > dim) return 0;
+    const uint64_t each = stride * KV_B * sizeof(float);
+    return heads * rows > DEC_KEPT / each ? DEC_KEPT + 1 : heads * rows * each;
+}
+
 int plan_decode(okf_ctx *c, DecArgs &a) {
-    const uint64_t rows = (uint64_t)a.tokens * (a.heads / a.c.heads), rpb = rows > 16 ? 32 : 16;
-    a.rb = (uint32_t)((rows + rpb - 1) / rpb);
-    const uint64_t base = (uint64_t)a.s.count * a.c.heads * a.rb;
+    const DecRows r(c, a.s.count, a.heads, a.c.heads, a.c.dim, a.tokens);
+    a.rb = (uint32_t)r.rb;
     const uint64_t span = a.window ? std::min<uint64_t>(((uint64_t)a.window + a.tokens) / KV_B + 2, a.s.stride) : a.s.stride;
-    auto up = [](uint64_t x, uint64_t y) { return (x + y - 1) / y; };
-    const uint64_t want = (uint64_t)c->cus * (a.c.dim <= 128 ? 2 : 1);
-    const uint64_t each = base * up(span, DEC_W) <= c->cus ? 1 : 2;
-    uint64_t splits = std::min(up(want, base), up(span, each * DEC_W));
-    if (a.s.count > 1) splits = std::max(splits, std::min(up(2 * want, base), up(span, 4 * DEC_W)));
+    const uint64_t each = r.base * up(span, DEC_W) <= c->cus ? 1 : 2;
+    uint64_t splits = std::min(up(r.want, r.base), up(span, each * DEC_W));
+    if (a.s.count > 1) splits = std::max(splits, std::min(up(2 * r.want, r.base), up(span, 4 * DEC_W)));
     splits = std::min<uint64_t>(splits, DEC_SPLITS);
-    auto bytes = [&](uint64_t n) {  // m and l, then partial outputs
-        return base * n * rpb * 2 * sizeof(float) + (n > 1 ? base * n * rpb * a.c.dim * sizeof(float) : 0);
-    };
-    // Scores kept for the weights, where that is less to write and read than the keys are to read
-    // again (8 sequences of up to 16000 tokens, 2 rows of 64: 31.6 us without) and the room is there.
-    const uint64_t kept = a.w_out && a.rb == 1 && rpb == 16 && 8 * rows <= a.c.dim
-                              ? base * rows * a.s.stride * KV_B * sizeof(float) : 0;
-    const uint64_t to = (bytes(splits) + 15) / 16 * 16;
+    auto bytes = [&](uint64_t n) { return r.bytes(r.base * n, a.c.dim, n > 1); };
+    const uint64_t kept = a.w_out ? dec_kept(r.base, r.rows, a.c.dim, a.s.stride) : 0, to = up(bytes(splits), 16) * 16;
     if (kept && kept <= DEC_KEPT && (to + kept <= c->part_bytes || grow_part(c, to + kept, true) == OKF_OK))
         a.sc = c->part + to / sizeof(float);
     else if (splits > 1 || a.w_out) {
@@ -129,9 +142,9 @@ int plan_decode(okf_ctx *c, DecArgs &a) {
     a.splits = (uint32_t)splits;
     if (splits > 1 || a.w_out) {
         a.ml = c->part;
-        a.part = c->part + base * splits * rpb * 2;
+        a.part = c->part + r.base * splits * r.rpb * 2;
     }
-    if (base * splits + 8ull * a.rb > 0xFFFFFFull) return OKF_E_SHAPE;
+    if (r.base * splits + 8 * r.rb > 0xFFFFFFull) return OKF_E_SHAPE;
     return OKF_OK;
 }
 
@@ -212,6 +225,29 @@ int okf_attn_decode(okf_ctx *c, const okf_kv_cache *cache, const okf_kv_seqs *se
     if (a.ml) note_capture(c, false, true, false);
     with_dims(cache->dim, [&](auto ks) { launch_decode<decltype(ks)::value>(c, a, rows > 16); });
     return finish(c);
+}
+
+int okf_attn_reserve(okf_ctx *c, uint32_t seqs, uint32_t stride, uint32_t heads, uint32_t kv_heads, uint32_t dim,
+                     uint32_t tokens, int32_t weights) {
+    if (!c) return OKF_E_ARG;
+    if (!seqs || !stride || !tokens || tokens > 65535 || !heads || heads > 65535 || !kv_heads || heads % kv_heads || !good_dim(dim))
+        return OKF_E_SHAPE;
+    const uint64_t sh = (uint64_t)seqs * kv_heads, group = heads / kv_heads;
+    if (sh * tokens * group > 0x3FFFFFFFull) return OKF_E_SHAPE;
+    if (c->device < 0) return OKF_E_NODEV;
+    (void)hipSetDevice(c->device);
+    // Of any smaller call, too: base blocks in up(2 want, base) splits are less than 2 want + base
+    // workgroups, and in a split for every DEC_W pages no more than that many; the scores are most
+    // with as many tokens as they are still kept for.
+    const DecRows r(c, seqs, heads, kv_heads, dim, tokens);
+    uint64_t need = up(r.bytes(std::min(2 * r.want + r.base, r.base * up(stride, DEC_W)), dim, true), 16) * 16;
+    const uint64_t most = std::min<uint64_t>(tokens, std::min(16u, dim / 8) / group);
+    if (weights && most) need += std::min(dec_kept(sh, most * group, dim, stride), DEC_KEPT);
+    const bool reserved = c->reserved;
+    c->reserved = false;
+    const int st = grow_part(c, need);
+    c->reserved = reserved;
+    return st;
 }
 
 int okf_kv_append(okf_ctx *c, const okf_kv_cache *cache, const okf_kv_seqs *seqs, const void *k, const void *v,

@@ -106,7 +106,8 @@ int okf_ctx_stream(okf_ctx *ctx, void **stream);
  * other formats uses the same scratch for its fp16 activations, and every
  * tile GEMM for its K-split partials, where they fit, and otherwise runs
  * without them: the activations rounded per tile, or one K range; the K
- * split changes only the order of the fp32 sums.)
+ * split changes only the order of the fp32 sums.  okf_attn_decode's splits:
+ * okf_attn_reserve.)
  * Without it the scratch grows on demand (hipMalloc after draining the
  * stream). */
 int okf_ctx_reserve(okf_ctx *ctx, uint64_t gemm_nk, uint32_t argmax_n, uint32_t argmax_rows);
@@ -331,12 +332,23 @@ int okf_kv_read(okf_ctx *ctx, const okf_kv_cache *cache, const okf_kv_seqs *seqs
  * values; w_in NULL counts as 0, w_in = w_out adds in place.
  * Scratch: the partial results of sequences split over workgroups, and with w_out
  * and few rows the scores (at most 256 MB; else they are computed twice), in the
- * context's buffer (see okf_ctx_reserve); where it may not grow, fewer splits and
+ * context's buffer (okf_attn_reserve); where it may not grow, fewer splits and
  * no scores (the order of the fp32 sums changes), and with w_out OKF_E_SHAPE if
  * not even one split fits. */
 int okf_attn_decode(okf_ctx *ctx, const okf_kv_cache *cache, const okf_kv_seqs *seqs, const float *q, float *o,
                     uint32_t tokens, uint32_t heads, float scale, uint32_t window, const float *w_in, float *w_out,
                     uint64_t w_stride);
+
+/* Allocates the scratch of okf_attn_decode up front: for up to seqs sequences
+ * with page table rows of up to stride entries, heads query heads over
+ * kv_heads kv heads of width dim, up to `tokens` tokens each, and any window;
+ * with `weights` nonzero for calls with w_out too.  Such calls then allocate
+ * nothing, and are split as on a context whose scratch grows, also on one that
+ * okf_ctx_reserve has fixed (before or after this call) and in a captured
+ * graph.  The buffer is the one of the argmax pairs and K-split partials: the
+ * largest of what is asked for, not the sum. */
+int okf_attn_reserve(okf_ctx *ctx, uint32_t seqs, uint32_t stride, uint32_t heads, uint32_t kv_heads, uint32_t dim,
+                     uint32_t tokens, int32_t weights);
 
 /* Cuts each sequence, per kv head, to `keep` tokens: its first `sink`, its
  * last `recent`, and of those between the ones of the largest weight w_in
