@@ -365,7 +365,8 @@ __global__ __launch_bounds__(S::NT, S::WAVES) void attn_prompt_kernel(AttnArgs a
     // A tile's weights from its scores.  The running maximum moves only when it is passed by a
     // factor of 2^8 (limit): weights of up to 256 lose nothing, and most tiles need no new factors.
     const float slack = 8.0f / c;
-    auto weights = [&](const floatx16 (&s)[TT], Weights &p) __attribute__((always_inline)) {
+    // (careful: see below)
+    auto weights = [&](const floatx16 (&s)[TT], Weights &p, auto careful) __attribute__((always_inline)) {
         float x = s[0][0];
 #pragma unroll
         for (int t = 0; t < TT; t++)
@@ -383,11 +384,13 @@ __global__ __launch_bounds__(S::NT, S::WAVES) void attn_prompt_kernel(AttnArgs a
             mc = (nm == -__builtin_inff() ? 0.0f : nm * c) - UP;
         }
         float l1 = 0;
+        [[maybe_unused]] const float ref = m == -__builtin_inff() ? 0.0f : m;
 #pragma unroll
         for (int t = 0; t < TT; t++)
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
-                const float e0 = __builtin_amdgcn_exp2f(fmaf(s[t][i], c, -mc)), e1 = __builtin_amdgcn_exp2f(fmaf(s[t][i + 1], c, -mc));
+                const float e0 = __builtin_amdgcn_exp2f(careful ? fmaf(s[t][i] - ref, c, UP) : fmaf(s[t][i], c, -mc));
+                const float e1 = __builtin_amdgcn_exp2f(careful ? fmaf(s[t][i + 1] - ref, c, UP) : fmaf(s[t][i + 1], c, -mc));
                 l += e0, l1 += e1;
                 const int kk = 2 * t + i / 8, at = i % 8 / 2;
                 if constexpr (NP == 1) {
@@ -439,7 +442,7 @@ __global__ __launch_bounds__(S::NT, S::WAVES) void attn_prompt_kernel(AttnArgs a
             Weights p;
             qk(kbuf(here), s);
             if (!is_whole(j)) mask(s, j);
-            weights(s, p);
+            weights(s, p, std::false_type{});
             pv(p, vbuf(here));
         };
         for (int n = 0; n < steps; n += 2) {
@@ -449,14 +452,17 @@ __global__ __launch_bounds__(S::NT, S::WAVES) void attn_prompt_kernel(AttnArgs a
     }
 
     // A value that is not finite makes NaN of rows that do not see it (0 * NaN), and an
-    // infinity's parts of a score; both show in the results.  Then the workgroup makes the
-    // pass again, carefully: such values key by key, such scores in fp32.
+    // infinity's parts of a score; both show in the results.  Where the maximum is large, its
+    // product's rounding (half of 2^-23 of it) is a factor of its own on all of a row's weights, up
+    // to one that no 16-bit, then no fp32 number holds.  Then the workgroup makes the pass again,
+    // carefully: such values key by key, such scores in fp32, weights from the scores' differences.
     float nan = l * 0.0f;
 #pragma unroll
     for (int d = 0; d < DT; d++)
 #pragma unroll
         for (int i = 0; i < 16; i++) nan = fmaf(o[d][i], 0.0f, nan);
-    if (__syncthreads_or(nan != 0)) {
+    const bool large = m > -__builtin_inff() && fabsf(m) * c >= 0x1p20f;
+    if (__syncthreads_or(nan != 0 || large)) {
         start();
 #pragma unroll 1
         for (int n = 0; n < steps; n++) {
@@ -489,7 +495,7 @@ __global__ __launch_bounds__(S::NT, S::WAVES) void attn_prompt_kernel(AttnArgs a
             const bool whole = is_whole(j);
             if (!whole) mask(s, j);
             Weights p;
-            weights(s, p);
+            weights(s, p, std::true_type{});
             bool bad = false;
             if (!whole) {
                 constexpr uint32_t EXP = __is_same(E, _Float16) ? 0x7C007C00u : 0x7F807F80u, ONE = __is_same(E, _Float16) ? 0x04000400u : 0x00800080u;

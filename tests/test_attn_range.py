@@ -42,6 +42,51 @@ def test_prompt_scale_of_any_size(enc, t):
         assert np.abs(got - ref).max() <= tol(q, k, v, scale * 4.0 ** e, n, D, t), e
 
 
+@gpu
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("scale", [1.0, -1.0, 0.5, 0.125])
+@pytest.mark.parametrize("H,n,before", [(2, 70, 100), (2, 60, 1000), (40, 900, 0)])
+def test_prompt_scores_at_the_types_ends(enc, t, scale, H, n, before):
+    """Keys whose scores are the type's lowest or highest value, as a mask or a bias within the keys
+    has them: alone they share the weight, beside others they take none or all of it."""
+    rng = np.random.default_rng(19)
+    D, m, top = 64, n + before, float(torch.finfo(TYPES[t]).max if t == "f16" else torch.finfo(torch.bfloat16).max)
+    q, k, v = np.zeros((n, H, D), np.float32), np.zeros((m, 1, D), np.float32), rng.standard_normal((m, 1, D)).astype(np.float32)
+    q[..., 0] = 1
+    usual = rng.standard_normal(m) * 3
+    for kind in ("lowest", "highest", "lowest and usual", "lowest first", "highest here and there", "both"):
+        k[:, 0, 0] = {"lowest": -top, "highest": top, "lowest and usual": np.where(rng.random(m) < 0.3, -top, usual),
+                      "lowest first": np.where(np.arange(m) < m // 2 + 3, -top, usual),
+                      "highest here and there": np.where(np.arange(m) % 97 == 50, top, usual),
+                      "both": np.where(np.arange(m) % 97 == 50, top, -top)}[kind]
+        q_, k_, v_ = (dev(x, TYPES[t]) for x in (q, k, v))
+        got = run_prompt(enc, q_, k_, v_, [0, n], [0, m], t, 0, scale, H, 1, D)
+        ref = ao.prompt(host(q_)[:, :1], host(k_), host(v_), [0, n], [0, m], 0, scale)  # (all heads alike)
+        small = np.where(np.abs(k) < 100, k, 0)
+        assert np.abs(got - ref).max() <= tol(q, small, v, abs(scale), m, D, t), kind
+
+
+@gpu
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("scale", [2.0 ** -4, 2.0 ** -2, 16.0, 256.0, 2.0 ** 12, 2.0 ** 30, 2.0 ** 90])
+@pytest.mark.parametrize("H,n,before", [(2, 70, 100), (2, 60, 1000), (40, 900, 0)])
+def test_prompt_large_scores(enc, t, sign, scale, H, n, before):
+    """Scores of sign 2^25 + 4 j, j < 16, which fp32 holds exactly, under scales that leave neighbours
+    some or no weight: exponents of up to 2^117.  Bound: the sums' u, a few u of the exponents that
+    still count (up to 30), and for f16 / bf16 a weight's and the output's half step."""
+    rng = np.random.default_rng(20)
+    D, m = 64, n + before
+    q, k, v = np.zeros((n, H, D), np.float32), np.zeros((m, 1, D), np.float32), rng.standard_normal((m, 1, D)).astype(np.float32)
+    q[..., 0], q[..., 1], k[..., 0] = 2048, 4, sign * 16384
+    k[:, 0, 1] = rng.integers(0, 16, m)
+    q_, k_, v_ = (dev(x, TYPES[t]) for x in (q, k, v))
+    got = run_prompt(enc, q_, k_, v_, [0, n], [0, m], t, 0, scale, H, 1, D)
+    ref = ao.prompt(host(q_)[:, :1], host(k_), host(v_), [0, n], [0, m], 0, scale)  # (all heads alike)
+    bound = (2 * m + 100) * 2.0 ** -24 + (0 if t == "f32" else torch.finfo(TYPES[t]).eps)
+    assert np.abs(got - ref).max() <= bound * np.abs(v).max()
+
+
 @pytest.mark.parametrize("over,status", [({"n_q": 0x7FFFFF00}, ok.OKF_E_NODEV), ({"n_q": 0x7FFFFF01}, ok.OKF_E_SHAPE),
                                          ({"n_k": 0x7FFFFF00}, ok.OKF_E_NODEV), ({"n_k": 0x7FFFFF01}, ok.OKF_E_SHAPE)])
 def test_prompt_rows_that_32_bits_hold(over, status):
