@@ -134,8 +134,11 @@ int plan_decode(okf_ctx *c, DecArgs &a) {
     if (kept && kept <= DEC_KEPT && (to + kept <= c->part_bytes || grow_part(c, to + kept, true) == OKF_OK))
         a.sc = c->part + to / sizeof(float);
     else if (splits > 1 || a.w_out) {
+        // (o over q: written by a launch behind the one that reads q again for the weights)
+        const uint64_t least = a.w_out && a.q == a.o ? 2 : 1;
+        splits = std::max(splits, least);
         if (bytes(splits) > c->part_bytes && grow_part(c, bytes(splits), true) != OKF_OK) {
-            while (splits > 1 && bytes(splits) > c->part_bytes) splits--;
+            while (splits > least && bytes(splits) > c->part_bytes) splits--;
             if (a.w_out && bytes(splits) > c->part_bytes) return OKF_E_SHAPE;
         }
     }
@@ -144,7 +147,7 @@ int plan_decode(okf_ctx *c, DecArgs &a) {
         a.ml = c->part;
         a.part = c->part + r.base * splits * r.rpb * 2;
     }
-    if (r.base * splits + 8 * r.rb > 0xFFFFFFull) return OKF_E_SHAPE;
+    if (r.base * splits + 8 * r.rb > 0xFFFFFFull || (splits > 1 && r.base / r.rb * r.rows > 0xFFFFFFull)) return OKF_E_SHAPE;
     return OKF_OK;
 }
 
@@ -161,10 +164,11 @@ void launch_decode_n(okf_ctx *c, const DecArgs &a) {
         hipLaunchKernelGGL(attn_dec_sum_kernel, dim3(joins + sh * parts), dim3(DEC_NT), 0, c->stream, a, parts, joins);
     } else if (a.w_out) {
         const uint32_t parts = std::max(1u, std::min(4 * c->cus / sh, (a.s.stride + DEC_W - 1) / DEC_W));
-        hipLaunchKernelGGL((attn_dec_weights_kernel<KS, NR>), dim3(joins + sh * parts), dim3(DEC_NT), 0, c->stream, a, parts, joins);
-    } else if (joins) {
-        hipLaunchKernelGGL(attn_dec_join_kernel, dim3(joins), dim3(DEC_NT), 0, c->stream, a, 16u * NR);
+        const uint32_t beside = a.q == a.o ? 0 : joins;
+        hipLaunchKernelGGL((attn_dec_weights_kernel<KS, NR>), dim3(beside + sh * parts), dim3(DEC_NT), 0, c->stream, a, parts, beside);
+        if (beside) return;
     }
+    if (joins && !a.sc) hipLaunchKernelGGL(attn_dec_join_kernel, dim3(joins), dim3(DEC_NT), 0, c->stream, a, 16u * NR);
 }
 
 template <int KS>
@@ -218,6 +222,10 @@ int okf_attn_decode(okf_ctx *c, const okf_kv_cache *cache, const okf_kv_seqs *se
     if (w_out && w_stride < (uint64_t)seqs->stride * KV_B) return OKF_E_SHAPE;
     const uint64_t sh = (uint64_t)seqs->count * cache->heads, rows = (uint64_t)tokens * (heads / cache->heads);
     if (sh * rows > 0x3FFFFFFFull) return OKF_E_SHAPE;
+    const uint64_t values = sh * rows * cache->dim;
+    if (q != o && rows_meet(q, values, values, o, values, values, 1)) return OKF_E_ARG;
+    const uint64_t row = (uint64_t)seqs->stride * KV_B;
+    if (w_in && w_in != w_out && rows_meet(w_in, w_stride, row, w_out, w_stride, row, sh)) return OKF_E_ARG;
     if ((st = begin(c))) return st;
     DecArgs a{cache_of(cache), seqs_of(seqs), q, o, tokens, heads, scale, window, w_in, w_out, w_stride, 1, 1,
               nullptr, nullptr, nullptr};
@@ -237,10 +245,11 @@ int okf_attn_reserve(okf_ctx *c, uint32_t seqs, uint32_t stride, uint32_t heads,
     if (c->device < 0) return OKF_E_NODEV;
     (void)hipSetDevice(c->device);
     // Of any smaller call, too: base blocks in up(2 want, base) splits are less than 2 want + base
-    // workgroups, and in a split for every DEC_W pages no more than that many; the scores are most
-    // with as many tokens as they are still kept for.
+    // workgroups, and in a split for every DEC_W pages no more than that many (two splits at least
+    // for weights with o over q); the scores are most with as many tokens as they are still kept for.
     const DecRows r(c, seqs, heads, kv_heads, dim, tokens);
-    uint64_t need = up(r.bytes(std::min(2 * r.want + r.base, r.base * up(stride, DEC_W)), dim, true), 16) * 16;
+    const uint64_t n = std::max(std::min(2 * r.want + r.base, r.base * up(stride, DEC_W)), weights ? 2 * r.base : 0);
+    uint64_t need = up(r.bytes(n, dim, true), 16) * 16;
     const uint64_t most = std::min<uint64_t>(tokens, std::min(16u, dim / 8) / group);
     if (weights && most) need += std::min(dec_kept(sh, most * group, dim, stride), DEC_KEPT);
     const bool reserved = c->reserved;

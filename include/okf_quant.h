@@ -329,7 +329,9 @@ int okf_kv_read(okf_ctx *ctx, const okf_kv_cache *cache, const okf_kv_seqs *seqs
  * result has fp32 precision.  With w_out, the attention weight that each
  * token got is added up: w_out[s][head][t] = w_in[s][head][t] + the sum over
  * the queries and the query heads of the kv head, t < len, rows of w_stride
- * values; w_in NULL counts as 0, w_in = w_out adds in place.
+ * values; w_in NULL counts as 0, w_in = w_out adds in place.  o may
+ * be q.  q and o, or w_in and w_out, that overlap in any other way are an
+ * OKF_E_ARG.
  * Scratch: the partial results of sequences split over workgroups, and with w_out
  * and few rows the scores (at most 256 MB; else they are computed twice), in the
  * context's buffer (okf_attn_reserve); where it may not grow, fewer splits and

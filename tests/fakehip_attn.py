@@ -15,10 +15,11 @@ def run(fake, steps, **env):
 
 
 class Child(fakehip._Child):
-    def decode(self, seqs, stride, heads, kv_heads, dim, tokens, weights, window=0):
+    def decode(self, seqs, stride, heads, kv_heads, dim, tokens, weights, window=0, over=False):
         cache = self.ok.KVCache(self.P, self.P, self.P, self.P, 100, kv_heads, dim)
         w = self.P if weights else None
-        self.enc.attn_decode(cache, self.ok.KVSeqs(self.P, self.P, seqs, stride), self.P, self.P, tokens, heads, 1.0, window=window,
+        o = self.P if over else self.P << 32  # (over the queries, or far from them)
+        self.enc.attn_decode(cache, self.ok.KVSeqs(self.P, self.P, seqs, stride), self.P, o, tokens, heads, 1.0, window=window,
                              w_in=w, w_out=w, w_stride=64 * stride)
 
     def attn_reserve(self, seqs, stride, heads, kv_heads, dim, tokens, weights):

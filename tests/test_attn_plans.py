@@ -22,7 +22,7 @@ def fake(tmp_path_factory):
 # (sequences, stride, heads, kv heads, width, tokens, weights)
 CALLS = [(1, 40, 4, 1, 64, 1, 1), (1, 1600, 20, 4, 256, 4, 0), (1, 1600, 20, 4, 256, 4, 1), (32, 128, 40, 8, 128, 1, 0),
          (32, 128, 40, 8, 128, 1, 1), (8, 250, 16, 8, 64, 1, 1), (3, 7, 5, 1, 80, 2, 1), (1, 32, 16, 8, 128, 1, 0),
-         (5, 999, 24, 8, 96, 1, 1), (64, 300, 64, 8, 128, 1, 1), (1, 100000, 8, 8, 128, 2, 1)]
+         (5, 999, 24, 8, 96, 1, 1), (64, 300, 64, 8, 128, 1, 1), (1, 100000, 8, 8, 128, 2, 1), (600, 1, 40, 1, 64, 1, 1), (1200, 2, 40, 1, 64, 1, 1)]
 
 
 @pytest.mark.parametrize("call", CALLS)
@@ -31,7 +31,7 @@ def test_reserved_as_grown(fake, call, order):
     """The plan of a context that grows, with nothing allocated, also for fewer sequences, tokens and pages."""
     seqs, stride, heads, kv, dim, tokens, w = call
     calls = [call, call[:6] + (0,), (1,) + call[1:], (seqs, max(1, stride // 3)) + call[2:], (max(1, seqs // 2),) + call[1:5] + (1, w),
-             call + (100,)]
+             call + (100,), call + (0, True), (seqs, 1) + call[2:] + (0, True)]
     reserve, fix = ["attn_reserve", *call], ["reserve", 1, 1, 1]
     before = {"first": [reserve, fix], "last": [fix, reserve], "alone": [reserve], "captured": [reserve, ["capture", 1]]}[order]
     steps = [["decode", *c] for c in calls if w or not c[6]]
@@ -137,3 +137,17 @@ def test_decode_plan(fake, call, splits, then):
     assert k["name"] == "attn_dec_kernel" and k["args"] == [(dim + 63) // 64, 2 if rows > 16 else 1]
     assert k["grid"][0] == -(-seqs * kv * splits // 8) * 8 * -(-rows // (32 if rows > 16 else 16))
     assert [v["name"] for v in rest] == ([then] if then else [])
+
+
+# o over q: written by the join behind the launch that reads q again for the weights.
+@pytest.mark.parametrize("call,names", [
+    ((600, 1, 40, 1, 64, 1, 1), ["attn_dec_kernel", "attn_dec_weights_kernel", "attn_dec_join_kernel"]),
+    ((1, 1563, 20, 4, 256, 4, 1), ["attn_dec_kernel", "attn_dec_weights_kernel", "attn_dec_join_kernel"]),
+    ((8, 250, 16, 8, 64, 1, 1), ["attn_dec_kernel", "attn_dec_sum_kernel"]), ((1, 4, 16, 8, 128, 1, 0), ["attn_dec_kernel"])])
+def test_decode_over_its_queries(fake, call, names):
+    (r,) = fakehip_attn.run(fake, [["decode", *call, 0, True]])
+    assert r["status"] == 0 and [v["name"] for v in r["launches"]] == names
+    rows, base = call[5] * call[2] // call[3], call[0] * call[3]
+    if "attn_dec_join_kernel" in names:
+        assert r["launches"][0]["grid"][0] >= 2 * base * -(-rows // (32 if rows > 16 else 16))
+        assert r["launches"][1]["grid"][0] == base * max(1, min(1024 // base, -(-call[1] // 4))) and r["launches"][2]["grid"][0] == base * rows
