@@ -17,16 +17,23 @@
 // as target), double-buffered; rows are read in an order such that 16-byte chunk c
 // of row r stands at c ^ at_fk(r) / at_fv(r), which spreads the reads of both
 // products over the banks.  fp32 inputs are split into three bf16 parts on their way
-// to LDS (x = x0 + x1 + x2 exactly, each part the next eight bits), and so are the
-// weights: six of the nine products of parts, the others are below 2^-22 of the
+// to LDS (x = x0 + x1 + x2 exactly from 2^-110 up, each part the next eight bits), and so
+// are the weights: six of the nine products of parts, the others are below 2^-22 of the
 // whole.
 //
-// Measured (MI355X): f16, 8192 rows x 40 heads of 128 700-740 us, 930-980 TFLOP/s; a matrix
-// product of 8192 in f16 runs at 1119 there, both at the 2.0 GHz or less that the card's
+// Measured (MI355X): f16, 8192 rows x 40 heads of 128 682-705 us, 975-1010 TFLOP/s; a matrix
+// product of 8192 in f16 runs at 1119-1157 there, both at the 2.0 GHz or less that the card's
 // power leaves.  Without its loads from memory the variant named at the pass took 14 %
 // less, without its reads of LDS 11 %: no one of matrix cores (57 % of their time), vector
-// units (50 %) and LDS bounds it alone.  8 packed bf16 prompts of up to 1111 x 16 heads 37 us; with the last
-// sequence's tiles first 47.
+// units (50 %) and LDS bounds it alone.  8 packed bf16 prompts of up to 1111 x 16 heads 34-36 us; with the
+// last sequence's tiles first 47.
+//
+// Registers: the second, careful pass is part of the kernel and sets what the first one
+// runs with.  A lane's (bf16, f16 alike; without that pass): 64 wide 186 to 190 (112 to 118), 128 wide
+// 237, and 256 with 3 spilled for 128 rows (156, 167), 256 wide 512 with 36 to 44 spilled (404, 439): one
+// wavefront a SIMD there, two elsewhere.  Widths that are not compiled for spill more: 68 for 112 with
+// 128 rows, 468 to 677 past 128.  fp32: two wavefronts a SIMD at up to 64 wide with 128 rows or
+// eight wavefronts, else one; 200 registers spilled at 256 wide, 1907 at the other widths past 128.
 #pragma once
 #include <type_traits>
 
@@ -394,6 +401,10 @@ __global__ __launch_bounds__(S::NT, S::WAVES) void attn_prompt_kernel(AttnArgs a
                 l += e0, l1 += e1;
                 const int kk = 2 * t + i / 8, at = i % 8 / 2;
                 if constexpr (NP == 1) {
+                    // (rounded to the inputs' type, half a step each: the second product at the first
+                    // one's rate.  Their sum is kept of the unrounded ones.  bf16 2.0e-3 from 64 bits, with
+                    // fp32 weights 1.6e-3, the output's own rounding; f16 2.8e-4 and 2.1e-4.  In two
+                    // parts the product would take twice as long.)
                     p.x[0][kk][at] = at_pack<E>(e0, e1);
                 } else {
                     uint32_t s0, s1, s2;

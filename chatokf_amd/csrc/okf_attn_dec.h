@@ -23,10 +23,11 @@
 // of a workgroup join their results at the end.
 //
 // Bound by the cache's bytes for batches (32 sequences of up to 8192 tokens, 8 kv heads of
-// 128: 56 us, 5.2 TB/s, as fast as a copy), by the chain of loads (length, page, scale, keys)
-// and the second launch for one short sequence (1999 tokens 7.3 + 3.6 us), by latency and the
-// vector units for wide heads (100003 tokens x 4 x 256, 20 rows each: 58 us, 3.5 TB/s: one
-// wavefront a SIMD; two, with the values in the keys' registers, spill: 100 us).
+// 128: this launch 56 us again and again on one cache, 5.2 TB/s, as fast as a copy; a call on a
+// cache not read before 69 us, 6 of them the join's), by the chain of loads (length, page, scale, keys)
+// and the second launch for one short sequence (1999 tokens 7.3 + 4.0 us), by latency and the
+// vector units for wide heads (100003 tokens x 4 x 256, 20 rows each: 57 us, the call 64, 3.2 TB/s:
+// one wavefront a SIMD; two, with the values in the keys' registers, spill: 100 us).
 #pragma once
 #include "okf_ffn_mfma.h"
 #include "okf_kv_seqs.h"

@@ -2,6 +2,14 @@
 prompt, an 8-bit paged KV cache, decode steps that add up attention weights, and
 eviction by them when the chat reaches its limit.
 
+Weights come from decode steps and verify passes alone: a prompt adds none.  A
+chat cut before its first step has equal weights for all tokens, so that its
+first tokens stay; one cut soon after, what the last steps looked at.
+
+Torch's own work (tensors made, filled, freed) belongs on the default stream,
+which the context's stream keeps in order with; on another one the caller waits
+where they meet.
+
 ``python -m chatokf_amd.session`` runs a layer with random weights through two
 prompt chunks and some steps, and prints what they took.
 """

@@ -258,8 +258,10 @@ int okf_embed_batch(okf_ctx *ctx, const okf_weight *w, const int32_t *ids, uint3
  * row does not see have no influence on it, NaN and infinities included.
  * Starts that leave [0, n_q] / [0, n_k] or decrease are clamped.  Scores,
  * sums and products are held in fp32; with f32 inputs the products keep
- * fp32 precision, with f16 / bf16 the softmax weights are rounded to that
- * type for the second product, and o once.  Scratch: none. */
+ * fp32 precision (inputs from 2^-110 up), with f16 / bf16 the softmax weights
+ * are rounded to that type for the second product, and o once.  Scores that
+ * fp32 holds are right up to its ends; values are summed up before the sum is
+ * divided by the weights', so they should stay below 2^100.  Scratch: none. */
 typedef struct {
     const void *q, *k, *v;          /* rows of heads x dim / kv_heads x dim values */
     void *o;                        /* n_q rows of heads x dim */
@@ -326,7 +328,9 @@ int okf_kv_read(okf_ctx *ctx, const okf_kv_cache *cache, const okf_kv_seqs *seqs
  * only the last `window` of them; one that sees none gives 0.  q and o:
  * fp32 [count][tokens][heads][dim], 16-byte aligned.  Codes enter the integer
  * matrix cores as they are; queries and weights as 23-bit integers, so the
- * result has fp32 precision.  With w_out, the attention weight that each
+ * result has fp32 precision, for queries, scales and page scales of any finite
+ * size whose scores stay below 2^127 and for values below 2^80 (they are summed
+ * up in units of 2^-23 of a weight).  With w_out, the attention weight that each
  * token got is added up: w_out[s][head][t] = w_in[s][head][t] + the sum over
  * the queries and the query heads of the kv head, t < len, rows of w_stride
  * values; w_in NULL counts as 0, w_in = w_out adds in place.  o may
