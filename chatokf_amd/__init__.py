@@ -30,6 +30,7 @@ EXPORTS = (
     "okf_gemv", "okf_gemv_silu", "okf_gemv_gate_up", "okf_ffn", "okf_silu_mul", "okf_gemm", "okf_gemm_tile", "okf_dequant_row",
     "okf_embed_batch", "okf_add_rmsnorm_batch", "okf_argmax_rows", "okf_argmax_rows_noalloc",
     "okf_stream_read", "okf_attn_prompt", "okf_attn_decode", "okf_attn_reserve", "okf_kv_append", "okf_kv_read", "okf_kv_evict",
+    "okf_norm_rope_rows", "okf_conv_rows", "okf_delta_step", "okf_delta_prompt", "okf_delta_reserve",
     "okf_parallel_begin",
     "okf_parallel_end", "okf_sync", "okf_set_fault_rate", "okf_last_hip_error", "okf_strerror",
     "okf_gguf_open", "okf_gguf_close", "okf_gguf_tensor_count", "okf_gguf_tensor_at", "okf_gguf_find",
@@ -84,6 +85,45 @@ class OkfKVSeqs(ctypes.Structure):
                 ("stride", ctypes.c_uint32)]
 
 
+class OkfRope(ctypes.Structure):
+    """``okf_rope`` of include/okf_quant.h."""
+    _fields_ = ([("rot", ctypes.c_uint32), ("pairs", ctypes.c_int32), ("base", ctypes.c_float), ("factor", ctypes.c_float),
+                 ("original", ctypes.c_uint32)] + [(n, ctypes.c_float) for n in ("beta_fast", "beta_slow", "mag")] +
+                [("div", ctypes.c_void_p)])
+
+
+class OkfNormRope(ctypes.Structure):
+    """``okf_norm_rope`` of include/okf_quant.h."""
+    _fields_ = (
+        [(n, ctypes.c_void_p) for n in ("q", "k", "q_out", "k_out")] + [("type", ctypes.c_int32)] +
+        [(n, ctypes.c_uint32) for n in ("heads", "kv_heads", "dim", "n")] +
+        [(n, ctypes.c_uint64) for n in ("q_stride", "k_stride", "q_out_stride", "k_out_stride", "q_head", "k_head", "q_out_head",
+                                        "k_out_head")] +
+        [("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p), ("eps", ctypes.c_float), ("pos", ctypes.c_void_p),
+         ("rope", OkfRope)])
+
+
+class OkfStateSeqs(ctypes.Structure):
+    """``okf_state_seqs`` of include/okf_quant.h."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("start", "slot")] + [(n, ctypes.c_uint32) for n in ("seqs", "n", "slots")] +
+                [(n, ctypes.c_void_p) for n in ("state_in", "state_out")])
+
+
+class OkfConv(ctypes.Structure):
+    """``okf_conv`` of include/okf_quant.h."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "y", "w", "bias")] + [("type", ctypes.c_int32), ("silu", ctypes.c_int32)] +
+                [("channels", ctypes.c_uint32), ("width", ctypes.c_uint32), ("x_stride", ctypes.c_uint64),
+                 ("y_stride", ctypes.c_uint64)])
+
+
+class OkfDelta(ctypes.Structure):
+    """``okf_delta`` of include/okf_quant.h."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "g", "beta", "o")] + [("type", ctypes.c_int32)] +
+                [(n, ctypes.c_uint32) for n in ("k_heads", "v_heads", "k_dim", "v_dim")] +
+                [(n, ctypes.c_uint64) for n in ("q_stride", "k_stride", "v_stride", "o_stride", "g_stride", "beta_stride")] +
+                [("scale", ctypes.c_float)])
+
+
 class OkfError(RuntimeError):
     def __init__(self, status: int, what: str):
         self.status = status
@@ -129,6 +169,11 @@ def _lib():
             "okf_kv_append": [vp, KC, KS, vp, vp, i32, vp, u32, u64, u64],
             "okf_kv_read": [vp, KC, KS, vp, vp, i32, vp, u32, u64, u64],
             "okf_kv_evict": [vp, KC, KS, KC, KS, u32, u32, u32, vp, u64, vp, u64, vp],
+            "okf_norm_rope_rows": [vp, ctypes.POINTER(OkfNormRope)],
+            "okf_conv_rows": [vp, ctypes.POINTER(OkfConv), ctypes.POINTER(OkfStateSeqs)],
+            "okf_delta_step": [vp, ctypes.POINTER(OkfDelta), ctypes.POINTER(OkfStateSeqs)],
+            "okf_delta_prompt": [vp, ctypes.POINTER(OkfDelta), ctypes.POINTER(OkfStateSeqs)],
+            "okf_delta_reserve": [vp, i32, u32, u32, u32, u32, u32, u32],
             "okf_parallel_begin": [vp],
             "okf_parallel_end": [vp],
             "okf_sync": [vp],
@@ -223,6 +268,19 @@ class KVSeqs:
         self._c = OkfKVSeqs(_ptr(pages), _ptr(lens), self.count, self.stride)
 
     def c(self) -> OkfKVSeqs:
+        return self._c
+
+
+class Rope:
+    """``okf_rope``: how the first ``rot`` dimensions of a head turn with the position (pairs: neighbours
+    instead of halves; div: a torch tensor of rot / 2 divisors in device memory, or None)."""
+
+    def __init__(self, rot: int, pairs: bool = False, base: float = 1e4, factor: float = 1.0, original: int = 0,
+                 beta_fast: float = 32.0, beta_slow: float = 1.0, mag: float = 0.0, div=None):
+        self.div = div
+        self._c = OkfRope(int(rot), int(pairs), base, factor, int(original), beta_fast, beta_slow, mag, _ptr(div))
+
+    def c(self) -> OkfRope:
         return self._c
 
 
@@ -407,6 +465,48 @@ class Enc:
                                            _ptr(w_in), w_in_stride, _ptr(w_out), w_out_stride, _ptr(kept)),
                     "okf_kv_evict")
 
+    def norm_rope(self, rope: Rope, pos, n: int, q, q_out, heads: int, k=None, k_out=None, kv_heads: int = 0, dim: int = 0,
+                  type: int = F32, q_norm=None, k_norm=None, eps: float = 0.0, strides=(0, 0, 0, 0), head_strides=(0, 0, 0, 0)):
+        """okf_norm_rope_rows: head norms (where given) and the rotation by pos; strides (of rows) and
+        head_strides of q, k, q_out, k_out in values, 0 for dense."""
+        r = OkfNormRope(_ptr(q), _ptr(k), _ptr(q_out), _ptr(k_out), int(type), heads, kv_heads, dim, n, *strides, *head_strides,
+                        _ptr(q_norm), _ptr(k_norm), eps, _ptr(pos), rope.c())
+        self._check(self._lib.okf_norm_rope_rows(self.h, ctypes.byref(r)), "okf_norm_rope_rows")
+
+    def conv(self, x, w, y, start, seqs: int, n: int, channels: int, width: int, type: int = F32, bias=None, silu: bool = False,
+             state_in=None, state_out=None, slot=None, slots: int = 0, strides=(0, 0)):
+        """okf_conv_rows: the causal convolution of each channel over packed sequences with their states
+        (slots: how many states there are, 0 for seqs); strides of x and y in values, 0 for dense."""
+        a = OkfConv(_ptr(x), _ptr(y), _ptr(w), _ptr(bias), int(type), int(silu), channels, width, *strides)
+        s = OkfStateSeqs(_ptr(start), _ptr(slot), seqs, n, slots or seqs, _ptr(state_in), _ptr(state_out))
+        self._check(self._lib.okf_conv_rows(self.h, ctypes.byref(a), ctypes.byref(s)), "okf_conv_rows")
+
+    def _delta(self, call, what, q, k, v, g, beta, out, start, seqs, n, k_heads, v_heads, k_dim, v_dim, type, scale, state_in, state_out,
+               slot, slots, strides, gate_strides):
+        d = OkfDelta(_ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(out), int(type), k_heads, v_heads, k_dim, v_dim, *strides,
+                     *gate_strides, scale)
+        s = OkfStateSeqs(_ptr(start), _ptr(slot), seqs, n, slots or seqs, _ptr(state_in), _ptr(state_out))
+        self._check(call(self.h, ctypes.byref(d), ctypes.byref(s)), what)
+
+    def delta_prompt(self, q, k, v, g, beta, out, start, seqs: int, n: int, k_heads: int, v_heads: int, k_dim: int, v_dim: int,
+                     type: int = F32, scale: float = 1.0, state_in=None, state_out=None, slot=None, slots: int = 0,
+                     strides=(0, 0, 0, 0), gate_strides=(0, 0)):
+        """okf_delta_prompt: the gated delta rule over packed sequences, their tokens in chunks; strides of q,
+        k, v, out and of g, beta in values, 0 for dense."""
+        self._delta(self._lib.okf_delta_prompt, "okf_delta_prompt", q, k, v, g, beta, out, start, seqs, n, k_heads, v_heads, k_dim, v_dim,
+                    type, scale, state_in, state_out, slot, slots, strides, gate_strides)
+
+    def delta_step(self, q, k, v, g, beta, out, start, seqs: int, n: int, k_heads: int, v_heads: int, k_dim: int, v_dim: int,
+                   type: int = F32, scale: float = 1.0, state_in=None, state_out=None, slot=None, slots: int = 0,
+                   strides=(0, 0, 0, 0), gate_strides=(0, 0)):
+        """okf_delta_step: the same token by token, for the few tokens of a decode step or a verify pass."""
+        self._delta(self._lib.okf_delta_step, "okf_delta_step", q, k, v, g, beta, out, start, seqs, n, k_heads, v_heads, k_dim, v_dim,
+                    type, scale, state_in, state_out, slot, slots, strides, gate_strides)
+
+    def delta_reserve(self, n: int, seqs: int, k_heads: int, v_heads: int, k_dim: int, v_dim: int, type: int = F32):
+        """okf_delta_reserve: allocate the scratch of delta_prompt calls of up to these sizes now."""
+        self._check(self._lib.okf_delta_reserve(self.h, int(type), n, seqs, k_heads, v_heads, k_dim, v_dim), "okf_delta_reserve")
+
     def reserve(self, gemm_nk: int, argmax_n: int, argmax_rows: int):
         """okf_ctx_reserve: allocate the scratch now; later calls allocate nothing."""
         self._check(self._lib.okf_ctx_reserve(self.h, int(gemm_nk), int(argmax_n), int(argmax_rows)),
@@ -514,5 +614,6 @@ class GGUF:
 __all__ = [
     "Q8_0", "Q4_K", "IQ2_XXS", "Q2_0", "Q4_0", "IQ4_NL", "Q5_K", "Q6_K", "IQ4_XS", "IQ2_XS", "IQ2_S", "IQ3_XXS", "IQ3_S",
     "IQ1_S", "IQ1_M", "F32", "F16", "BF16", "Q2_K", "Q3_K", "NAMES", "BY_NAME", "block_elems", "row_bytes",
-    "QuantTensor", "KVCache", "KVSeqs", "KV_BLOCK", "OkfAttn", "OkfKVCache", "OkfKVSeqs", "Enc", "OkfError", "OkfWeight", "OkfGGUFTensor", "GGUF", "lib", "EXPORTS", "LIB_PATH",
+    "QuantTensor", "KVCache", "KVSeqs", "KV_BLOCK", "Rope", "OkfAttn", "OkfKVCache", "OkfKVSeqs", "OkfRope", "OkfNormRope",
+    "OkfStateSeqs", "OkfConv", "OkfDelta", "Enc", "OkfError", "OkfWeight", "OkfGGUFTensor", "GGUF", "lib", "EXPORTS", "LIB_PATH",
 ]

@@ -17,11 +17,12 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
-# the C ABI (okf_quant.hip; attention and the KV cache in okf_attn.hip) and one
-# translation unit per type of prompt attention (okf_attn_*.hip) and per group of
-# formats (okf_fmt_*.hip), compiled in parallel and linked into one library
-SRCS = ([os.path.join(CSRC, "okf_quant.hip")] + sorted(glob.glob(os.path.join(CSRC, "okf_attn*.hip"))) +
-        sorted(glob.glob(os.path.join(CSRC, "okf_fmt_*.hip"))))
+# the C ABI (okf_quant.hip; attention and the KV cache in okf_attn.hip, what stands
+# around the projections in okf_layer.hip) and one translation unit per type of
+# prompt attention (okf_attn_*.hip) and of the delta rule (okf_delta_*.hip) and per
+# group of formats (okf_fmt_*.hip), compiled in parallel and linked into one library
+SRCS = ([os.path.join(CSRC, "okf_quant.hip"), os.path.join(CSRC, "okf_layer.hip")] +
+        [p for kind in ("attn", "delta", "fmt") for p in sorted(glob.glob(os.path.join(CSRC, f"okf_{kind}*.hip")))])
 LIB = os.path.join(HERE, "libokf_quant.so")
 OBJ = os.path.join(HERE, "_build")
 LIB_TRACE = os.path.join(HERE, "libokf_quant_trace.so")

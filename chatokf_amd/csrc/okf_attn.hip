@@ -1,6 +1,7 @@
 // okf_attn.hip -- the C ABI of attention and the KV cache (include/okf_quant.h)
 // over okf_attn.h, okf_attn_dec.h and okf_kv.h.
 #include "okf_impl.h"
+#include "okf_args.h"
 #include "okf_attn_run.h"
 #include "okf_attn_dec.h"
 #include "okf_kv.h"
@@ -9,18 +10,6 @@ namespace {
 
 using namespace okf;
 using namespace okf_impl;
-
-bool aligned4(const void *p) { return ((uintptr_t)p & 3) == 0; }
-
-bool attn_type(int32_t t) { return t == F32 || t == F16 || t == BF16; }
-
-// Runs f with a value of the element type t (attn_type).
-template <class Fn>
-void with_type(int32_t t, Fn f) {
-    if (t == F32) f(float{});
-    else if (t == F16) f(_Float16{});
-    else f(__bf16{});
-}
 
 // Runs f with the 64s of dimensions that hold dim, as a constant.
 template <class Fn>
@@ -32,8 +21,6 @@ void with_dims(uint32_t dim, Fn f) {
     default: f(std::integral_constant<int, 4>{}); break;
     }
 }
-
-bool good_dim(uint32_t d) { return d >= 16 && d <= 256 && d % 16 == 0; }
 
 int check_cache(const okf_kv_cache *c) {
     if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) return OKF_E_ARG;
@@ -50,12 +37,6 @@ int check_seqs(const okf_kv_seqs *s) {
 
 KvCache cache_of(const okf_kv_cache *c) { return {c->k, c->v, c->k_scale, c->v_scale, c->pages, c->heads, c->dim}; }
 KvSeqs seqs_of(const okf_kv_seqs *s) { return {s->pages, s->len, s->count, s->stride}; }
-
-// A row stride of 16-byte rows: `least` values when 0, else at least that and whole 16 bytes.
-bool row_stride(uint64_t &st, uint64_t least, uint32_t size) {
-    if (!st) st = least;
-    return st >= least && st <= (1ull << 40) && st * size % 16 == 0;
-}
 
 // Whether n rows of la values, sa apart, share memory with n rows of lb values, sb apart.
 bool rows_meet(const float *a, uint64_t sa, uint64_t la, const float *b, uint64_t sb, uint64_t lb, uint64_t n) {

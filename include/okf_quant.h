@@ -372,6 +372,124 @@ int okf_kv_evict(okf_ctx *ctx, const okf_kv_cache *src, const okf_kv_seqs *from,
                  const okf_kv_seqs *to, uint32_t keep, uint32_t sink, uint32_t recent, const float *w_in,
                  uint64_t w_in_stride, float *w_out, uint64_t w_out_stride, int32_t *kept);
 
+/* ------------------------------------------- around the projections --
+ * What a hybrid model's two kinds of layers compute beside their projections
+ * and attention: head norms with the rotation by positions, and the gated delta
+ * rule's layer (the short convolution and the rule itself).  The reference
+ * computes these in its engines; these entry points have layouts of their own. */
+
+/* The angles of a rotation by positions.  Pair i of rot / 2 turns by
+ * pos * f_i, f_i = base^(-2 i / rot) / div[i].  With original = 0 all f_i are divided by
+ * `factor`; else (a context of `original` positions stretched `factor` times) pair i's
+ * becomes f_i (r_i / factor + 1 - r_i), r_i = (i - low) / max(high - low, 0.001) inside
+ * [0, 1], low = floor(d(beta_fast)) but at least 0, high = ceil(d(beta_slow)) but at most
+ * rot - 1, d(t) = rot ln(original / (2 pi t)) / (2 ln base).  Sines and cosines are
+ * multiplied by `mag`; 0 stands for 1, or for 0.1 ln(factor) + 1 with original > 0 and
+ * factor > 1.  Angles are formed in 64 bits and reduced there: far positions are as
+ * exact as near ones. */
+typedef struct {
+    uint32_t rot;          /* dimensions that turn, the first of a head: even; 0: none */
+    int32_t pairs;         /* 0: dimension i with i + rot / 2; 1: 2 i with 2 i + 1 */
+    float base;            /* above 0; with original > 0 above 1 */
+    float factor;          /* above 0; 1: positions as they are */
+    uint32_t original;
+    float beta_fast, beta_slow; /* turns in the original context; above 0 (with original > 0 only) */
+    float mag;
+    const float *div;      /* device memory, rot / 2 values; NULL: ones */
+} okf_rope;
+
+/* Norms and rotation of queries and keys, head by head, in one pass: for each of the n
+ * rows and each head, y = x * norm / sqrt(mean(x^2) + eps) where that norm is not NULL,
+ * then the rotation of y's first rot dimensions by the row's position; the others stay.
+ * fp32 inside, rounded once to `type`.  k may be NULL (heads of one kind).  With norms
+ * of dim^-0.5 and eps / dim for eps this is x / sqrt(sum(x^2) + eps), the delta rule's
+ * unit vectors.  q_out may be q and k_out k, with the same strides; other overlaps of
+ * outputs with inputs or each other are an OKF_E_ARG (so are ranges that lie inside each
+ * other's rows with row strides that differ). */
+typedef struct {
+    const void *q, *k;              /* rows of heads x dim / kv_heads x dim values */
+    void *q_out, *k_out;
+    int32_t type;                   /* OKF_TYPE_F32, _F16 or _BF16 */
+    uint32_t heads, kv_heads, dim;  /* dim: a multiple of 16 up to 256 */
+    uint32_t n;                     /* rows, up to 2^31 - 256 */
+    uint64_t q_stride, k_stride, q_out_stride, k_out_stride;    /* values from a row to the next (0: dense) */
+    uint64_t q_head, k_head, q_out_head, k_out_head;            /* values from a head to the next (0: dim) */
+    const float *q_norm, *k_norm;   /* dim weights, or NULL */
+    float eps;
+    const int32_t *pos;             /* device memory, n positions (any int32); may be NULL with rot = 0 */
+    okf_rope rope;
+} okf_norm_rope;
+/* Pointers are 16-byte aligned (pos, norms and div 4), strides whole multiples of 16 bytes. */
+int okf_norm_rope_rows(okf_ctx *ctx, const okf_norm_rope *r);
+
+/* Packed sequences that carry a state: sequence s has the rows [start[s], start[s + 1])
+ * (starts that leave [0, n] or decrease are clamped) and the state slot[s] of `slots`
+ * (slot NULL: s).  It begins from state_in's, or from zeros where state_in is NULL, and
+ * what it leaves goes to state_out's, where that is not NULL; a sequence without rows
+ * leaves its state as it began.  state_out may be state_in; it may not overlap it in any other way
+ * (OKF_E_ARG).  A slot outside [0, slots) begins from zeros and is not kept; two
+ * sequences may share a slot only to begin from it (state_out NULL), else what is left
+ * there is either's or a mixture.  Slots of no sequence stay as they are. */
+typedef struct {
+    const int32_t *start;           /* device memory, seqs + 1 */
+    const int32_t *slot;            /* device memory, seqs, or NULL */
+    uint32_t seqs, n, slots;        /* sequences, rows in all (up to 2^31 - 256), slots (at least seqs with slot NULL) */
+    const void *state_in;
+    void *state_out;
+} okf_state_seqs;
+
+/* The short causal convolution of every channel: y[t][c] = act(bias[c] + the sum over
+ * j < width of w[c][j] x[t - width + 1 + j][c]), act the identity or silu(x) = x / (1 +
+ * exp(-x)); rows before a sequence's first are its state's, [slot][width - 1][channels]
+ * of `type`, the oldest first.  fp32 inside, y rounded once; states are copied.  y may not
+ * overlap x (OKF_E_ARG). */
+typedef struct {
+    const void *x;                  /* n rows of `channels` values */
+    void *y;
+    const float *w, *bias;          /* [channels][width]; [channels] or NULL */
+    int32_t type;                   /* OKF_TYPE_F32, _F16 or _BF16 */
+    int32_t silu;
+    uint32_t channels, width;       /* width 2 .. 8 */
+    uint64_t x_stride, y_stride;    /* values from a row to the next (0: dense) */
+} okf_conv;
+int okf_conv_rows(okf_ctx *ctx, const okf_conv *a, const okf_state_seqs *s);
+
+/* The gated delta rule: value head h's state S [k_dim][v_dim] (fp32, [slot][v_heads][k_dim]
+ * [v_dim]) takes each token as
+ *   S = exp(g) S;  S += k (beta (v - S^T k))^T;  o = scale S^T q
+ * with the queries and keys of key head h / (v_heads / k_heads).  Keys of length about
+ * one and beta in [0, 2] keep it stable; nothing here normalizes them (okf_norm_rope_rows).
+ * g may be -inf: the state is cleared before the token.  All sums are in fp32 or with
+ * fp32's precision, for values between 2^-100 and 2^100; o is rounded once. */
+typedef struct {
+    const void *q, *k, *v;          /* rows of k_heads x k_dim, k_heads x k_dim, v_heads x v_dim values */
+    const float *g, *beta;          /* rows of v_heads values */
+    void *o;                        /* rows of v_heads x v_dim; may be v, with its stride */
+    int32_t type;                   /* of q, k, v and o: OKF_TYPE_F32, _F16 or _BF16 */
+    uint32_t k_heads, v_heads;      /* v_heads a multiple of k_heads */
+    uint32_t k_dim, v_dim;          /* multiples of 16 up to 256 */
+    uint64_t q_stride, k_stride, v_stride, o_stride, g_stride, beta_stride; /* values from a row to the next (0: dense) */
+    float scale;
+} okf_delta;
+/* Pointers are 16-byte aligned (g and beta 4), strides of q, k, v and o whole multiples
+ * of 16 bytes.  o may not overlap the inputs in any other way (OKF_E_ARG).
+ *
+ * okf_delta_step goes token by token with the state in registers: decode steps and
+ * verify passes.  Scratch: none.  okf_delta_prompt is for many tokens: the sequences in chunks whose
+ * tokens are solved for together.  It gives the same results but for the order of fp32
+ * sums.  Scratch: what the chunks' products need (okf_delta_reserve), in the context's
+ * buffer; where that may not grow, fewer chunks at a time, and where not even few fit it
+ * goes token by token. */
+int okf_delta_step(okf_ctx *ctx, const okf_delta *d, const okf_state_seqs *s);
+int okf_delta_prompt(okf_ctx *ctx, const okf_delta *d, const okf_state_seqs *s);
+
+/* Allocates the scratch of okf_delta_prompt up front for up to n rows of up to seqs
+ * sequences: such calls then allocate nothing and run as on a context whose scratch grows,
+ * also on one that okf_ctx_reserve has fixed and in a captured graph.  It is the
+ * buffer of okf_attn_reserve: the largest of what is asked for, not the sum. */
+int okf_delta_reserve(okf_ctx *ctx, int32_t type, uint32_t n, uint32_t seqs, uint32_t k_heads, uint32_t v_heads, uint32_t k_dim,
+                      uint32_t v_dim);
+
 /* Waits for all work on the context's stream: the analogue of
  * commit + waitUntilCompleted (LLM/Base/MetalGates.swift:144-149).  Returns
  * OKF_E_HIP if a kernel failed. */
