@@ -83,13 +83,14 @@ __global__ __launch_bounds__(DS_NT) void delta_step_kernel(const DeltaArgs a) {
         floatx4 u;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            u[j] = beta * (vt[j] - e * dl_sum16(kr[j]));
-            qr[j] = (e * dl_sum16(qr[j]) + kq * u[j]) * a.scale;
+            kr[j] = dl_sum16(kr[j]), qr[j] = dl_sum16(qr[j]);
+            u[j] = beta * (vt[j] - (e == 0 ? 0.0f : e * kr[j]));
+            qr[j] = ((e == 0 ? 0.0f : e * qr[j]) + kq * u[j]) * a.scale;
         }
 #pragma unroll
         for (int i = 0; i < RK; i++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) S[i][j] = fmaf(kt[i], u[j], e * S[i][j]);
+            for (int j = 0; j < 4; j++) S[i][j] = fmaf(kt[i], u[j], e == 0 ? 0.0f : e * S[i][j]);
         if (rg == 0) {
             typedef T vec __attribute__((ext_vector_type(4)));
             vec x;

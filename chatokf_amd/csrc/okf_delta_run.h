@@ -2,7 +2,7 @@
 // okf_delta_<type>.hip, so that they compile in parallel.
 #pragma once
 #include "okf_impl.h"
-#include "okf_delta.h"
+#include "okf_delta_scan.h"
 
 namespace okf_impl {
 
@@ -14,12 +14,31 @@ void launch_delta_step(okf_ctx *c, const okf::DeltaArgs &a) {
     hipLaunchKernelGGL((okf::delta_step_kernel<T, RK>), dim3((uint32_t)((waves + 3) / 4)), dim3(okf::DS_NT), 0, c->stream, a);
 }
 
+// The chunks p.c0 .. p.c1 - 1: what each of them needs, then one behind the other.
+template <class T, int KS = 1>
+void launch_delta_chunks(okf_ctx *c, const okf::ScanArgs &p) {
+    using namespace okf;
+    if constexpr (KS < 8)
+        if (p.a.k_dim > 32 * KS) return launch_delta_chunks<T, KS + 1>(c, p);
+    constexpr uint32_t waves = DP_NT / 64;
+    const uint32_t tasks = (p.c1 - p.c0) * p.a.k_heads * p.passes;
+    hipLaunchKernelGGL((delta_prepare_kernel<T, KS>), dim3((tasks + waves - 1) / waves), dim3(DP_NT), 0, c->stream, p);
+    static std::atomic<uint64_t> attr{0};
+    set_lds_attr(c, (const void *)delta_scan_kernel<T, KS>, attr);
+    const uint32_t grid = p.a.s.count * p.a.v_heads * ((p.a.v_dim / 16 + 1) / 2);
+    hipLaunchKernelGGL((delta_scan_kernel<T, KS>), dim3(grid), dim3(DN_NT), dl_scan_lds<KS>(), c->stream, p);
+}
+
 #ifndef OKF_DELTA_TYPE
 extern template void launch_delta_step<float>(okf_ctx *, const okf::DeltaArgs &);
 extern template void launch_delta_step<_Float16>(okf_ctx *, const okf::DeltaArgs &);
 extern template void launch_delta_step<__bf16>(okf_ctx *, const okf::DeltaArgs &);
+extern template void launch_delta_chunks<float>(okf_ctx *, const okf::ScanArgs &);
+extern template void launch_delta_chunks<_Float16>(okf_ctx *, const okf::ScanArgs &);
+extern template void launch_delta_chunks<__bf16>(okf_ctx *, const okf::ScanArgs &);
 #else
 template void launch_delta_step<OKF_DELTA_TYPE>(okf_ctx *, const okf::DeltaArgs &);
+template void launch_delta_chunks<OKF_DELTA_TYPE>(okf_ctx *, const okf::ScanArgs &);
 #endif
 
 }  // namespace okf_impl

@@ -109,6 +109,48 @@ int run_step(okf_ctx *c, int32_t type, const DeltaArgs &a) {
     return finish(c);
 }
 
+// The chunks of okf_delta_prompt: how many there may be, how many at a time (their scratch in
+// DELTA_WORK bytes, a grid of less than 2^32 threads), and the bytes of a chunk and of two states
+// that go from one launch to the next.
+constexpr uint64_t DELTA_WORK = 512ull << 20;
+struct DeltaPlan {
+    uint64_t chunks, at_once, per_chunk, carry;
+    uint32_t kq, passes;
+    DeltaPlan(int32_t type, uint32_t n, uint32_t seqs, uint32_t k_heads, uint32_t v_heads, uint32_t k_dim, uint32_t v_dim) {
+        kq = dl_kq_bytes(type == F32 ? 3 : type == F16 ? 2 : 1, k_dim);
+        passes = (v_heads / k_heads + 1) / 2;
+        per_chunk = (uint64_t)k_heads * kq + (uint64_t)v_heads * DV_BYTES;
+        carry = 2ull * v_heads * k_dim * v_dim * sizeof(float);
+        chunks = std::min<uint64_t>(n, n / DC + (uint64_t)seqs);
+        at_once = std::min<uint64_t>(std::max<uint64_t>(DELTA_WORK / per_chunk, 1), (1u << 24) / (k_heads * passes));
+        at_once = std::min(std::max<uint64_t>(at_once, 1), chunks);
+    }
+    uint64_t bytes(uint64_t n) const { return carry + n * per_chunk; }
+};
+
+int run_prompt(okf_ctx *c, int32_t type, const DeltaArgs &a) {
+    DeltaPlan pl(type, a.s.n, a.s.count, a.k_heads, a.v_heads, a.k_dim, a.v_dim);
+    const uint64_t blocks = (uint64_t)a.s.count * a.v_heads * ((a.v_dim / 16 + 1) / 2);
+    if (blocks > 0xFFFFFFull) return run_step(c, type, a);
+    uint64_t n = pl.at_once;
+    if (pl.bytes(n) > c->part_bytes && grow_part(c, pl.bytes(n), true) != OKF_OK) {
+        n = c->part_bytes > pl.carry ? std::min((c->part_bytes - pl.carry) / pl.per_chunk, n) : 0;
+        if (n < std::min<uint64_t>(pl.at_once, 16)) return run_step(c, type, a);
+    }
+    note_capture(c, false, true, false);
+    float *carry = c->part;
+    const uint64_t state = pl.carry / 2 / sizeof(float);
+    ScanArgs p{a, (uint8_t *)(carry + 2 * state), pl.per_chunk, pl.kq, pl.passes, 0, 0, carry, carry + state};
+    for (uint64_t at = 0; at < pl.chunks; at += n) {
+        p.c0 = (uint32_t)at, p.c1 = (uint32_t)std::min(at + n, pl.chunks);
+        with_type(type, [&](auto t) { launch_delta_chunks<decltype(t)>(c, p); });
+        const float *out = p.carry_out;
+        p.carry_out = (float *)p.carry_in;
+        p.carry_in = out;
+    }
+    return finish(c);
+}
+
 }  // namespace
 
 extern "C" {
@@ -229,7 +271,7 @@ int okf_delta_prompt(okf_ctx *c, const okf_delta *d, const okf_state_seqs *s) {
     int st = check_delta(d, s, a);
     if (st) return st;
     if ((st = begin(c))) return st;
-    return run_step(c, d->type, a);
+    return run_prompt(c, d->type, a);
 }
 
 int okf_delta_reserve(okf_ctx *c, int32_t type, uint32_t n, uint32_t seqs, uint32_t k_heads, uint32_t v_heads, uint32_t k_dim,
@@ -240,7 +282,13 @@ int okf_delta_reserve(okf_ctx *c, int32_t type, uint32_t n, uint32_t seqs, uint3
         !good_dim(v_dim))
         return OKF_E_SHAPE;
     if (c->device < 0) return OKF_E_NODEV;
-    return OKF_OK;
+    (void)hipSetDevice(c->device);
+    const DeltaPlan pl(type, n, seqs, k_heads, v_heads, k_dim, v_dim);
+    const bool reserved = c->reserved;
+    c->reserved = false;
+    const int st = grow_part(c, pl.bytes(pl.at_once));
+    c->reserved = reserved;
+    return st;
 }
 
 }  // extern "C"

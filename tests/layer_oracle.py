@@ -59,7 +59,7 @@ def delta(q, k, v, g, beta, state, scale):
         for t in range(len(v)):
             for h in range(v.shape[1]):
                 kt, qt, e = k[t, h // G].astype(np.float64), q[t, h // G].astype(np.float64), np.exp(np.float64(g[t, h]))
-                S[h] = S[h] * e if e else np.where(np.isnan(S[h]), S[h], 0.0)
+                S[h] = S[h] * e if e else np.zeros_like(S[h])
                 S[h] += np.outer(kt, beta[t, h] * (v[t, h] - kt @ S[h]))
                 o[t, h] = qt @ S[h] * scale
     return o, S
