@@ -73,7 +73,7 @@ bool states_apart(const okf_state_seqs *s, uint64_t each) {
 
 StateSeqs seqs_of(const okf_state_seqs *s) { return {s->start, s->slot, s->seqs, s->n, s->slots}; }
 
-int check_delta(const okf_delta *d, const okf_state_seqs *s, DeltaArgs &a) {
+int check_delta(const okf_delta *d, const okf_state_seqs *s, DeltaArgs &a, bool over_v) {
     if (!d || !d->q || !d->k || !d->v || !d->g || !d->beta || !d->o) return OKF_E_ARG;
     int st = check_states(s);
     if (st) return st;
@@ -98,7 +98,7 @@ int check_delta(const okf_delta *d, const okf_state_seqs *s, DeltaArgs &a) {
     if (!apart(d->q, a.qs * size, kw * size) || !apart(d->k, a.ks * size, kw * size) || !apart(d->g, a.gs * 4, d->v_heads * 4) ||
         !apart(d->beta, a.bs * 4, d->v_heads * 4))
         return OKF_E_ARG;
-    if (!(d->o == d->v && a.os == a.vs) && !apart(d->v, a.vs * size, vw * size)) return OKF_E_ARG;
+    if (!(over_v && d->o == d->v && a.os == a.vs) && !apart(d->v, a.vs * size, vw * size)) return OKF_E_ARG;
     // (grids of less than 2^32 threads)
     if ((uint64_t)s->seqs * d->v_heads * (d->v_dim / 16) > 0x3FFFFFFull - 8) return OKF_E_SHAPE;
     return OKF_OK;
@@ -140,7 +140,8 @@ int run_prompt(okf_ctx *c, int32_t type, const DeltaArgs &a) {
     note_capture(c, false, true, false);
     float *carry = c->part;
     const uint64_t state = pl.carry / 2 / sizeof(float);
-    ScanArgs p{a, (uint8_t *)(carry + 2 * state), pl.per_chunk, pl.kq, pl.passes, 0, 0, carry, carry + state};
+    uint8_t *work = (uint8_t *)(carry + 2 * state);
+    ScanArgs p{a, work, work + n * a.k_heads * pl.kq, pl.kq, pl.passes, 0, 0, (uint32_t)n, carry, carry + state};
     for (uint64_t at = 0; at < pl.chunks; at += n) {
         p.c0 = (uint32_t)at, p.c1 = (uint32_t)std::min(at + n, pl.chunks);
         with_type(type, [&](auto t) { launch_delta_chunks<decltype(t)>(c, p); });
@@ -260,7 +261,7 @@ int okf_conv_rows(okf_ctx *c, const okf_conv *p, const okf_state_seqs *s) {
 
 int okf_delta_step(okf_ctx *c, const okf_delta *d, const okf_state_seqs *s) {
     DeltaArgs a;
-    int st = check_delta(d, s, a);
+    int st = check_delta(d, s, a, true);
     if (st) return st;
     if ((st = begin(c))) return st;
     return run_step(c, d->type, a);
@@ -268,7 +269,7 @@ int okf_delta_step(okf_ctx *c, const okf_delta *d, const okf_state_seqs *s) {
 
 int okf_delta_prompt(okf_ctx *c, const okf_delta *d, const okf_state_seqs *s) {
     DeltaArgs a;
-    int st = check_delta(d, s, a);
+    int st = check_delta(d, s, a, false);
     if (st) return st;
     if ((st = begin(c))) return st;
     return run_prompt(c, d->type, a);

@@ -464,7 +464,7 @@ int okf_conv_rows(okf_ctx *ctx, const okf_conv *a, const okf_state_seqs *s);
 typedef struct {
     const void *q, *k, *v;          /* rows of k_heads x k_dim, k_heads x k_dim, v_heads x v_dim values */
     const float *g, *beta;          /* rows of v_heads values */
-    void *o;                        /* rows of v_heads x v_dim; may be v, with its stride */
+    void *o;                        /* rows of v_heads x v_dim; for okf_delta_step it may be v, with its stride */
     int32_t type;                   /* of q, k, v and o: OKF_TYPE_F32, _F16 or _BF16 */
     uint32_t k_heads, v_heads;      /* v_heads a multiple of k_heads */
     uint32_t k_dim, v_dim;          /* multiples of 16 up to 256 */

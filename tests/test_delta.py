@@ -44,8 +44,8 @@ def detached():
     ({"state_out": FAR + 8}, ok.OKF_E_SHAPE), ({"strides": (127, 0, 0, 0)}, ok.OKF_E_SHAPE), ({"strides": (0, 130, 0, 0)}, ok.OKF_E_SHAPE),
     ({"strides": (0, 132, 0, 0)}, ok.OKF_E_NODEV), ({"strides": (0, 132, 0, 0), "type": ok.F16}, ok.OKF_E_SHAPE), ({"gate_strides": (3, 0)}, ok.OKF_E_SHAPE),
     ({"gate_strides": (5, 2 ** 41)}, ok.OKF_E_SHAPE), ({"gate_strides": (5, 9)}, ok.OKF_E_NODEV),
-    # overlaps: over v is fine, with another stride or a place in it not; over q, k or the gates never; columns of the same rows are
-    ({"out": FAKE * 4}, ok.OKF_E_NODEV), ({"out": FAKE * 4, "strides": (0, 0, 0, 516)}, ok.OKF_E_ARG), ({"out": FAKE * 4 + 16}, ok.OKF_E_ARG),
+    # overlaps: a step's over v is fine, with another stride or a place in it not; over q, k or the gates never; columns of the same rows are
+    ({"out": FAKE * 4}, {"step": ok.OKF_E_NODEV, "prompt": ok.OKF_E_ARG}), ({"out": FAKE * 4, "strides": (0, 0, 0, 516)}, ok.OKF_E_ARG), ({"out": FAKE * 4 + 16}, ok.OKF_E_ARG),
     ({"out": FAKE}, ok.OKF_E_ARG), ({"out": FAKE * 2}, ok.OKF_E_ARG), ({"out": FAKE * 8 - 16}, ok.OKF_E_ARG), ({"out": FAKE * 16 - 4080}, ok.OKF_E_ARG),
     ({"v": FAKE + 1024, "k": FAKE + 512, "out": FAKE + 3072, "strides": (1280,) * 4}, ok.OKF_E_NODEV),
     ({"v": FAKE + 1024, "k": FAKE + 512, "out": FAKE + 3056, "strides": (1280,) * 4}, ok.OKF_E_ARG),
@@ -54,7 +54,7 @@ def detached():
 def test_refusals(detached, form, over, status):
     a = dict(q=FAKE, k=FAKE * 2, v=FAKE * 4, g=FAKE * 8, beta=FAKE * 16, out=FAKE * 32, start=FAKE, seqs=2, n=7, k_heads=2, v_heads=4, k_dim=64,
              v_dim=128)
-    fails(lambda: calls(detached, form)(**{**a, **over}), status)
+    fails(lambda: calls(detached, form)(**{**a, **over}), status[form] if isinstance(status, dict) else status)
 
 
 def test_reserve_refusals(detached):
@@ -149,7 +149,8 @@ def test_places(enc, form, t):
     check(enc, form, Case(t, 1, 2, 64, 64, lens, slots=9), slot=[8, 0, 3, 5, 2], inplace=True)
     check(enc, form, Case(t, 1, 2, 64, 64, lens, slots=6), slot=[5, -1, 3, 6, 2 ** 31 - 1], inplace=True)
     check(enc, form, Case(t, 1, 2, 64, 64, lens, slots=6), slot=[5, 5, 5, 5, 0], keep=False)
-    check(enc, form, Case(t, 1, 2, 64, 64, lens), over_v=True)
+    if form == "step":
+        check(enc, form, Case(t, 1, 2, 64, 64, lens), over_v=True)
 
 
 @gpu
@@ -312,11 +313,12 @@ def test_offsets_past_32_bits(enc, form):
     pool[[slots - 1, 7]] = c.state
     ref = [c.want(i, host(c.state)[i], 0.25) for i in range(2)]
     st = 1 << 30
-    v = torch.empty(4 * st + VH * DV, dtype=torch.float32, device="cuda")
-    rows = torch.as_strided(v, (5, VH, DV), (st, DV, 1))
-    rows.copy_(c.v)
-    calls(enc, form)(c.q, c.k, v, c.g, c.beta, v, ints(c.start), 2, 5, 1, VH, DK, DV, scale=0.25, state_in=pool, state_out=pool,
+    v = torch.empty(4 * st + 2 * VH * DV, dtype=torch.float32, device="cuda")
+    rows = torch.as_strided(v, (5, 2, VH, DV), (st, VH * DV, DV, 1))
+    rows[:, 0].copy_(c.v)
+    calls(enc, form)(c.q, c.k, v, c.g, c.beta, v[VH * DV:], ints(c.start), 2, 5, 1, VH, DK, DV, scale=0.25, state_in=pool, state_out=pool,
                      slot=ints([slots - 1, 7]), slots=slots, strides=(0, 0, st, st))
+    rows = rows[:, 1]
     enc.sync()
     for i, at in enumerate((slots - 1, 7)):
         s, b = c.bounds(i, host(c.state)[i], ref[i][0], 0.25)
