@@ -33,24 +33,27 @@ __device__ __forceinline__ float dl_sum_rows(float x) {
     const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
-// Sum over the 16 lanes of the same l % 4, in every one of them.
-__device__ __forceinline__ float dl_sum16(float x) {
-    x += dl_lane<0x128>(x);
-    x += dl_lane<0x124>(x);
+// Sum over the lanes of the same l % CQ, in every one of them.
+template <int CQ>
+__device__ __forceinline__ float dl_sum_groups(float x) {
+    x += dl_lane<0x128>(x);  // (rows of 16 lanes turned by 8, by 4)
+    if constexpr (CQ == 4) x += dl_lane<0x124>(x);
     return dl_sum_rows(x);
 }
 
 constexpr int DS_NT = 256;
 
-// A wavefront holds 16 columns of one head's state, four a lane, over its 16 lanes of
-// RK = k_dim / 16 rows each.  Bound by the state's bytes: 64 KB in and 64 KB out for a head of 128 x 128.
-template <class T, int RK>
+// A wavefront holds 4 CQ columns of one head's state, four a lane, over its 64 / CQ lanes of
+// RK = k_dim CQ / 64 rows each.  Bound by the state's bytes: 64 KB in and 64 KB out for a head of 128 x 128.
+template <class T, int CQ, int RK>
 __global__ __launch_bounds__(DS_NT) void delta_step_kernel(const DeltaArgs a) {
-    const uint32_t lane = threadIdx.x & 63, rg = lane >> 2, tiles = a.v_dim / 16;
+    const uint32_t lane = threadIdx.x & 63, rg = lane / CQ, tiles = (a.v_dim + 4 * CQ - 1) / (4 * CQ);
     const uint32_t w = blockIdx.x * (DS_NT / 64) + (threadIdx.x >> 6);
     const uint32_t tile = w % tiles, h = w / tiles % a.v_heads, s = w / tiles / a.v_heads;
     if (s >= a.s.count) return;
-    const uint32_t col = tile * 16 + (lane & 3) * 4, kh = h / (a.v_heads / a.k_heads), row0 = rg * RK;
+    // (columns past the last: the last's again, not written)
+    const uint32_t place = (tile * CQ + lane % CQ) * 4, col = min(place, a.v_dim - 4), kh = h / (a.v_heads / a.k_heads), row0 = rg * RK;
+    const bool on = place < a.v_dim;
     const uint2 r = kv_rows(a.s.start, s, a.s.n);
     const int64_t slot = a.s.state(s);
     floatx4 S[RK];
@@ -79,11 +82,11 @@ __global__ __launch_bounds__(DS_NT) void delta_step_kernel(const DeltaArgs a) {
 #pragma unroll
             for (int j = 0; j < 4; j++) kr[j] = fmaf(kt[i], S[i][j], kr[j]), qr[j] = fmaf(qt[i], S[i][j], qr[j]);
         }
-        kq = dl_sum16(kq);
+        kq = dl_sum_groups<CQ>(kq);
         floatx4 u;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            kr[j] = dl_sum16(kr[j]), qr[j] = dl_sum16(qr[j]);
+            kr[j] = dl_sum_groups<CQ>(kr[j]), qr[j] = dl_sum_groups<CQ>(qr[j]);
             u[j] = beta * (vt[j] - (e == 0 ? 0.0f : e * kr[j]));
             qr[j] = ((e == 0 ? 0.0f : e * qr[j]) + kq * u[j]) * a.scale;
         }
@@ -91,7 +94,7 @@ __global__ __launch_bounds__(DS_NT) void delta_step_kernel(const DeltaArgs a) {
         for (int i = 0; i < RK; i++)
 #pragma unroll
             for (int j = 0; j < 4; j++) S[i][j] = fmaf(kt[i], u[j], e == 0 ? 0.0f : e * S[i][j]);
-        if (rg == 0) {
+        if (rg == 0 && on) {
             typedef T vec __attribute__((ext_vector_type(4)));
             vec x;
 #pragma unroll
@@ -99,7 +102,7 @@ __global__ __launch_bounds__(DS_NT) void delta_step_kernel(const DeltaArgs a) {
             *(vec *)(o + t * a.os) = x;
         }
     }
-    if (a.so && slot >= 0) {
+    if (a.so && slot >= 0 && on) {
 #pragma unroll
         for (int i = 0; i < RK; i++) *(floatx4 *)(a.so + at + (uint64_t)i * a.v_dim) = S[i];
     }

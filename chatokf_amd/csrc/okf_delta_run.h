@@ -6,12 +6,18 @@
 
 namespace okf_impl {
 
+// 16 columns a wavefront, or 32, whose rows are whole lines of 128 bytes, where those still leave
+// DS_WAVES wavefronts a CU.
+constexpr uint32_t DS_WAVES = 8;
 template <class T, int RK = 1>
 void launch_delta_step(okf_ctx *c, const okf::DeltaArgs &a) {
     if constexpr (RK < 16)
         if (a.k_dim != 16 * RK) return launch_delta_step<T, RK + 1>(c, a);
-    const uint64_t waves = (uint64_t)a.s.count * a.v_heads * (a.v_dim / 16);
-    hipLaunchKernelGGL((okf::delta_step_kernel<T, RK>), dim3((uint32_t)((waves + 3) / 4)), dim3(okf::DS_NT), 0, c->stream, a);
+    const uint64_t heads = (uint64_t)a.s.count * a.v_heads, wide = heads * ((a.v_dim + 31) / 32), narrow = heads * (a.v_dim / 16);
+    if (wide >= (uint64_t)DS_WAVES * c->cus)
+        hipLaunchKernelGGL((okf::delta_step_kernel<T, 8, 2 * RK>), dim3((uint32_t)((wide + 3) / 4)), dim3(okf::DS_NT), 0, c->stream, a);
+    else
+        hipLaunchKernelGGL((okf::delta_step_kernel<T, 4, RK>), dim3((uint32_t)((narrow + 3) / 4)), dim3(okf::DS_NT), 0, c->stream, a);
 }
 
 // The chunks p.c0 .. p.c1 - 1: what each of them needs, then one behind the other.

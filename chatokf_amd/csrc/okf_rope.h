@@ -81,6 +81,7 @@ template <class T, int L, bool CROSS>
 __global__ __launch_bounds__(RP_NT) void norm_rope_kernel(const RopeArgs a) {
     constexpr uint32_t V = 16 / sizeof(T), G = 64 / L;
     __shared__ float2 turns[RP_NT / 64][128];
+    __shared__ __align__(16) float norms[2][256];
     __shared__ float cross[CROSS ? RP_NT / 64 : 1][CROSS ? 64 * 2 * V : 1];
     const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63, u = lane % L;
     const uint32_t w = blockIdx.x * (RP_NT / 64) + wave, half = a.rot / 2;
@@ -93,6 +94,13 @@ __global__ __launch_bounds__(RP_NT) void norm_rope_kernel(const RopeArgs a) {
         d0 = u < hc ? u * V : 2 * u * V;
         d1 = u < hc ? d0 + half : d0 + V;
     }
+    // the norms' weights, once for the workgroup's rows
+    for (uint32_t i = threadIdx.x; i < 2 * a.dim; i += RP_NT) {
+        const float *nw = i < a.dim ? a.qn : a.kn;
+        if (nw) norms[i >= a.dim][i < a.dim ? i : i - a.dim] = nw[i < a.dim ? i : i - a.dim];
+    }
+    __syncthreads();
+    const float per_dim = 1.0f / (float)a.dim;
     const uint32_t turning = half > u * V ? min(half - u * V, V) : 0;
     for (uint32_t row = w / a.wpr; row < a.n; row += step) {
         if (a.rot) {
@@ -115,20 +123,22 @@ __global__ __launch_bounds__(RP_NT) void norm_rope_kernel(const RopeArgs a) {
             const bool on = mine && head < (key ? a.kv : a.heads);
             const T *x = key ? (const T *)a.k + row * a.ks + head * a.kh : (const T *)a.q + row * a.qs + head * a.qh;
             T *y = key ? (T *)a.ko + row * a.kos + head * a.koh : (T *)a.qo + row * a.qos + head * a.qoh;
-            const float *nw = key ? a.kn : a.qn;
             float v[2 * V], g[2 * V];
 #pragma unroll
             for (uint32_t j = 0; j < 2 * V; j++) v[j] = 0.0f;
             if (on) rp_load(x + d0, v), rp_load(x + d1, v + V);
-            if (nw) {
-                if (mine) {
+            if (key ? a.kn : a.qn) {
+                const float *nw = norms[key];
 #pragma unroll
-                    for (uint32_t j = 0; j < V; j++) g[j] = nw[d0 + j], g[V + j] = nw[d1 + j];
+                for (uint32_t j = 0; j < V; j += 4) {
+                    const floatx4 x0 = *(const floatx4 *)(nw + (mine ? d0 : 0) + j), x1 = *(const floatx4 *)(nw + (mine ? d1 : 0) + j);
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; i++) g[j + i] = x0[i], g[V + j + i] = x1[i];
                 }
                 float ss = 0;
 #pragma unroll
                 for (uint32_t j = 0; j < 2 * V; j++) ss = fmaf(v[j], v[j], ss);
-                const float r = 1.0f / sqrtf(rp_sum<L>(ss) / (float)a.dim + a.eps);
+                const float r = __builtin_amdgcn_rsqf(fmaf(rp_sum<L>(ss), per_dim, a.eps));  // (right to one step)
 #pragma unroll
                 for (uint32_t j = 0; j < 2 * V; j++) v[j] = v[j] * r * g[j];
             }
@@ -148,21 +158,17 @@ __global__ __launch_bounds__(RP_NT) void norm_rope_kernel(const RopeArgs a) {
                         v[j] = low ? v[j] * c.x - o * c.y : o * c.y + v[j] * c.x;
                     }
                 }
-            } else if (a.pairs) {
+            } else if (turning) {  // (a lane's pairs turn, but for those that the end of rot cuts off)
+                auto turn = [&](float &x0, float &x1, uint32_t j) {
+                    const float y0 = x0 * cs[j].x - x1 * cs[j].y, y1 = x0 * cs[j].y + x1 * cs[j].x;
+                    if (j < turning) x0 = y0, x1 = y1;
+                };
+                if (a.pairs) {
 #pragma unroll
-                for (uint32_t j = 0; j < V; j++) {
-                    const float x0 = v[2 * j], x1 = v[2 * j + 1];
-                    const bool on_j = j < turning;
-                    v[2 * j] = on_j ? x0 * cs[j].x - x1 * cs[j].y : x0;
-                    v[2 * j + 1] = on_j ? x0 * cs[j].y + x1 * cs[j].x : x1;
-                }
-            } else {
+                    for (uint32_t j = 0; j < V; j++) turn(v[2 * j], v[2 * j + 1], j);
+                } else {
 #pragma unroll
-                for (uint32_t j = 0; j < V; j++) {
-                    const float x0 = v[j], x1 = v[V + j];
-                    const bool on_j = j < turning;
-                    v[j] = on_j ? x0 * cs[j].x - x1 * cs[j].y : x0;
-                    v[V + j] = on_j ? x0 * cs[j].y + x1 * cs[j].x : x1;
+                    for (uint32_t j = 0; j < V; j++) turn(v[j], v[V + j], j);
                 }
             }
             if (on) rp_store(y + d0, v), rp_store(y + d1, v + V);
