@@ -478,8 +478,8 @@ typedef struct {
  * verify passes.  Scratch: none.  okf_delta_prompt is for many tokens: the sequences in chunks whose
  * tokens are solved for together.  It gives the same results but for the order of fp32
  * sums.  Scratch: what the chunks' products need (okf_delta_reserve), in the context's
- * buffer; where that may not grow, fewer chunks at a time, and where not even few fit it
- * goes token by token. */
+ * buffer; where that may not grow, fewer chunks at a time, and where not even few fit, or
+ * there are no more than 16 rows, it goes token by token. */
 int okf_delta_step(okf_ctx *ctx, const okf_delta *d, const okf_state_seqs *s);
 int okf_delta_prompt(okf_ctx *ctx, const okf_delta *d, const okf_state_seqs *s);
 

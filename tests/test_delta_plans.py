@@ -23,7 +23,7 @@ def fake(tmp_path_factory):
 
 # (type, rows, sequences, key heads, value heads, widths)
 PROMPTS = [("f32", 202, 2, 16, 16, 128, 128), ("bf16", 8192, 1, 16, 48, 128, 128), ("f16", 5000, 8, 16, 32, 128, 128), ("f32", 512, 1, 16, 48, 64, 128),
-           ("f32", 1, 1, 1, 1, 16, 16), ("bf16", 9, 4000, 2, 6, 80, 96), ("f32", 100000, 3, 16, 48, 256, 128), ("f16", 70000, 70000, 1, 1, 32, 16)]
+           ("f32", 17, 1, 1, 1, 16, 16), ("bf16", 40, 4000, 2, 6, 80, 96), ("f32", 100000, 3, 16, 48, 256, 128), ("f16", 70000, 70000, 1, 1, 32, 16)]
 
 
 @pytest.mark.parametrize("call", PROMPTS)
@@ -68,6 +68,12 @@ def test_scratch_that_may_not_grow(fake):
     assert r[1]["status"] == 0 and [x["name"] for x in r[1]["launches"]] == ["delta_step_kernel"]
     r = fakehip_delta.run(fake, [["attn_reserve", 32, 128, 40, 8, 128, 1, 1], FIX, call])
     assert r[2]["status"] == 0 and r[2]["launches"][0]["name"] == "delta_prepare_kernel" and r[2]["allocs"] == r[1]["allocs"]
+
+
+@pytest.mark.parametrize("seqs", [1, 5, 30])
+def test_few_rows_go_token_by_token(fake, seqs):
+    r = fakehip_delta.run(fake, [["delta", "prompt", "bf16", n, seqs, 2, 4, 64, 64] for n in (1, 16, 17)] + [["delta", "step", "bf16", 16, seqs, 2, 4, 64, 64]])
+    assert r[0]["launches"] == r[1]["launches"] == r[3]["launches"] and [x["name"] for x in r[2]["launches"]] == ["delta_prepare_kernel", "delta_scan_kernel"]
 
 
 def test_reserved_while_captured(fake):
