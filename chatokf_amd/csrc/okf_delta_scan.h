@@ -38,8 +38,8 @@ __host__ __device__ constexpr uint32_t dl_kq_bytes(int parts, uint32_t k_dim) { 
 
 struct ScanArgs {
     DeltaArgs a;
-    uint8_t *k_work, *v_work;  // of the chunks c0 .. c1 - 1: [k_heads][at_once][kq], [v_heads][at_once][DV_BYTES], so that a head's lie
-                               // side by side (a chunk's heads side by side: every chunk on another page, 417 us for 390)
+    uint8_t *k_work, *v_work;  // of the chunks c0 .. c1 - 1: [k_heads][at_once][kq], [v_heads][at_once][DV_BYTES]: a head's
+                               // chunks, which a workgroup goes through, side by side
     uint32_t kq, passes;       // passes: pairs of value heads of a key head
     uint32_t c0, c1, at_once;
     const float *carry_in;  // the state of the sequence that chunk c0 - 1 belongs to
@@ -243,7 +243,7 @@ __global__ __launch_bounds__(DP_NT) void delta_prepare_kernel(const ScanArgs p) 
         beta = a.beta[(uint64_t)(first + j) * a.bs + vh + half];
     }
     floatx4 kk[3] = {}, qk[3] = {};  // earlier and later tokens of tiles (0, 0), (0, 1), (1, 1)
-#pragma unroll 2
+#pragma unroll 1
     for (int ks = 0; ks < KS; ks++) {
         bf16x8d kp[2][NP], qp[2][NP];
 #pragma unroll
@@ -700,7 +700,7 @@ __global__ __launch_bounds__(DN_NT, KS * dl_parts<T>() <= 6 ? 2 : 1) void delta_
             for (int mt = 0; mt < 2; mt++) o[mt] = dl_mma(pp[mt], part, o[mt] * eg[mt]);
             fix();
             load_p(next);
-T *to = (T *)a.o + (uint64_t)(first + 4 * h) * a.os + vh * a.v_dim + col;
+            T *to = (T *)a.o + (uint64_t)(first + 4 * h) * a.os + vh * a.v_dim + col;
             if (left >= DC) {
 #pragma unroll
                 for (uint32_t j = 0; j < 8; j++) to[(j / 4 * 16 + j % 4) * a.os] = (T)(o[j / 4][j % 4] * a.scale);
