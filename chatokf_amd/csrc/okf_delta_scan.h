@@ -473,6 +473,9 @@ __global__ __launch_bounds__(DN_NT, KS * dl_parts<T>() <= 6 ? 2 : 1) void delta_
                 for (int i = 0; i < 4; i++) S[dt][i] = from && dt * 16 < (int)a.k_dim ? from[at + (uint64_t)(dt * 16 + i) * a.v_dim] : 0.0f;
         };
         load_state();
+        // Operands of wide fp32 keys do not fit in registers beside each other: there K^T is loaded while T R is made and K when
+        // K^T is used up (2048 tokens, 16 heads of 256 x 256: 465 us for 750; 192 dimensions, which fit, 259 for 253).
+        constexpr bool LATE = KS * NP > 18;
         bf16x8d ka[2][KS][NP], tp[2][3], kt[2 * KS][NP];
         floatx4 eg[2], el[2], v[2], ks0[2];
         float e_last;
@@ -556,10 +559,11 @@ __global__ __launch_bounds__(DN_NT, KS * dl_parts<T>() <= 6 ? 2 : 1) void delta_
         };
         if (n) {
             wait();
-            load_k(0), load_eg(0), load_t(0), load_kt(0);
+            load_k(0), load_eg(0), load_t(0);
+            if (!LATE) load_kt(0);
             read_state(0);
             wait();
-            load_k(min(1u, n - 1));
+            if (!LATE) load_k(min(1u, n - 1));
             dl_meet();  // (the first values)
             load_v(0);
         }
@@ -569,6 +573,7 @@ __global__ __launch_bounds__(DN_NT, KS * dl_parts<T>() <= 6 ? 2 : 1) void delta_
             floatx4 u[2];
             bf16x8d part[3];
             auto scale = [&](int dt) { S[dt] *= e_last; };
+            if (LATE) load_kt(c);
             // R = V - e^G K S and its parts; T R, the state's decay beside it
             constexpr int EARLY = KS;  // (decays until K S is there)
 #pragma unroll
@@ -611,9 +616,10 @@ __global__ __launch_bounds__(DN_NT, KS * dl_parts<T>() <= 6 ? 2 : 1) void delta_
             dl_meet();
             load_v(c + 1);
             dl_zip<2 * KS, 0>(by_kt(2), [](int) {});
-            load_kt(next);
+            if (LATE) load_k(next);
+            else load_kt(next);
             read_state(c + 1);
-            load_k(min(c + 2, n - 1));
+            if (!LATE) load_k(min(c + 2, n - 1));
         }
         if (n) {
             dl_meet();  // (the outputs are written)
