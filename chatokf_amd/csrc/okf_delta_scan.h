@@ -421,12 +421,17 @@ __device__ __forceinline__ void dl_meet() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+// Two wavefronts a SIMD where the registers of one fit in half of them (192 bf16 dimensions, which nearly do: 352 us for 440
+// with 8 sequences of 2048 tokens, 16 heads; 160 dimensions, which do: 489 for 376 at 32 heads if they had all).
+template <class T, int KS>
+constexpr bool dl_two() { return KS * dl_parts<T>() <= 6 && KS < 6; }
+
 // A workgroup takes 32 columns of a value head's state through its sequence's chunks, two wavefronts 16 of
 // them.  The first carries the state from chunk to chunk; the second makes the outputs from the
 // state's parts and the corrections that the first leaves in LDS, and brings it the values.  They meet once a
 // chunk, when its corrections are there.
 template <class T, int KS>
-__global__ __launch_bounds__(DN_NT, KS * dl_parts<T>() <= 6 ? 2 : 1) void delta_scan_kernel(const ScanArgs p) {
+__global__ __launch_bounds__(DN_NT, (dl_two<T, KS>() ? 2 : 1)) void delta_scan_kernel(const ScanArgs p) {
     constexpr int NP = dl_parts<T>();
     const DeltaArgs &a = p.a;
     extern __shared__ __align__(16) uint8_t dn_mem[];
