@@ -2,7 +2,9 @@
 // their states (okf_conv_rows): y[t] = act(b + sum_j w[j] x[t - W + 1 + j]).
 //
 // Bound by memory: a value is read once (the W - 1 rows in front of a block of CV_T once
-// more) and written once, 2 W + 4 operations for each.
+// more) and written once, 2 W + 4 operations for each.  7036 rows of 10240 bf16 channels, width 4, SiLU: 80 us, 3.7 TB/s
+// in and out; the vector units are half busy there, with conversions, products and SiLU, and the waits are what is left.
+// 32 sequences of one fp32 row: 5.4 us, the search for the sequence and two loads behind each other.
 #pragma once
 #include "okf_kv_seqs.h"
 

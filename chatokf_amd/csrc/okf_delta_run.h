@@ -7,7 +7,8 @@
 namespace okf_impl {
 
 // 16 columns a wavefront, or 32, whose rows are whole lines of 128 bytes, where those still leave
-// DS_WAVES wavefronts a CU.
+// DS_WAVES wavefronts a CU (32 sequences of 48 heads of 128 x 128: 43 us for 50; one sequence, spread
+// over half the CUs: 5.2 for 4.8).
 constexpr uint32_t DS_WAVES = 8;
 template <class T, int RK = 1>
 void launch_delta_step(okf_ctx *c, const okf::DeltaArgs &a) {

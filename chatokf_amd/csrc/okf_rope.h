@@ -2,8 +2,9 @@
 // the same pass (okf_norm_rope_rows).
 //
 // y = R(pos) (x w / sqrt(mean(x^2) + eps)): the norm's sum goes over a head, R turns the
-// pairs of its first rot dimensions.  All bound by memory: every value is read once and
-// written once, some 8 operations for each.
+// pairs of its first rot dimensions.  Bound by memory: every value is read once and
+// written once, some 8 operations for each.  8192 rows of 40 + 8 bf16 heads of 128 with norms: 43 us, 4.7 TB/s in
+// and out (a large copy 5.15); one row of 16 + 8 fp32 heads 3.5 us, the launch and a chain of two loads.
 #pragma once
 #include "okf_kv_seqs.h"
 
