@@ -54,6 +54,7 @@ __global__ __launch_bounds__(256) void conv_kernel(const ConvArgs a) {
     if (it.seq >= a.s.count || c >= a.channels) return;
     const uint2 r = kv_rows(a.s.start, it.seq, a.s.n);
     const uint32_t first = r.x + it.at * CV_T, last = min(first + CV_T, r.y);
+    if (it.at && first >= r.y) return;  // (not with starts that rise)
     const int64_t slot = a.s.state(it.seq);
     const T *x = (const T *)a.x + c;
     T *y = (T *)a.y + c;

@@ -230,6 +230,7 @@ __global__ __launch_bounds__(DP_NT) void delta_prepare_kernel(const ScanArgs p) 
     if (it.seq >= a.s.count) return;
     const uint2 r = kv_rows(a.s.start, it.seq, a.s.n);
     const uint32_t first = r.x + it.at * DC, n = min(r.y - first, DC);
+    if (first >= r.y) return;  // (not with starts that rise)
     bf16x8d *kq = (bf16x8d *)(p.k_work + ((uint64_t)kh * p.at_once + (chunk - p.c0)) * p.kq);
     auto vb = [&](uint32_t head) { return p.v_work + ((uint64_t)head * p.at_once + (chunk - p.c0)) * DV_BYTES; };
     const T *q = (const T *)a.q + kh * a.k_dim, *k = (const T *)a.k + kh * a.k_dim;

@@ -71,6 +71,11 @@ bool states_apart(const okf_state_seqs *s, uint64_t each) {
     return rows_apart(s->state_in, each, each, s->slots, s->state_out, each, each, s->slots);
 }
 
+// Whether states of `each` bytes share no memory with n rows of `row` bytes that the call reads or writes.
+bool state_apart(const void *state, const okf_state_seqs *s, uint64_t each, const void *p, uint64_t stride, uint64_t row) {
+    return !state || rows_apart(state, each, each, s->slots, p, stride, row, s->n);
+}
+
 StateSeqs seqs_of(const okf_state_seqs *s) { return {s->start, s->slot, s->seqs, s->n, s->slots}; }
 
 int check_delta(const okf_delta *d, const okf_state_seqs *s, DeltaArgs &a, bool over_v) {
@@ -99,6 +104,11 @@ int check_delta(const okf_delta *d, const okf_state_seqs *s, DeltaArgs &a, bool 
         !apart(d->beta, a.bs * 4, d->v_heads * 4))
         return OKF_E_ARG;
     if (!(over_v && d->o == d->v && a.os == a.vs) && !apart(d->v, a.vs * size, vw * size)) return OKF_E_ARG;
+    auto kept_apart = [&](const void *p, uint64_t stride, uint64_t row) { return state_apart(s->state_out, s, each, p, stride, row); };
+    if (!kept_apart(d->o, a.os * size, vw * size) || !state_apart(s->state_in, s, each, d->o, a.os * size, vw * size) ||
+        !kept_apart(d->q, a.qs * size, kw * size) || !kept_apart(d->k, a.ks * size, kw * size) || !kept_apart(d->v, a.vs * size, vw * size) ||
+        !kept_apart(d->g, a.gs * 4, d->v_heads * 4) || !kept_apart(d->beta, a.bs * 4, d->v_heads * 4))
+        return OKF_E_ARG;
     // (grids of less than 2^32 threads)
     if ((uint64_t)s->seqs * d->v_heads * (d->v_dim / 16) > 0x3FFFFFFull - 8) return OKF_E_SHAPE;
     return OKF_OK;
@@ -135,10 +145,12 @@ int run_prompt(okf_ctx *c, int32_t type, const DeltaArgs &a) {
     DeltaPlan pl(type, a.s.n, a.s.count, a.k_heads, a.v_heads, a.k_dim, a.v_dim);
     const uint64_t blocks = (uint64_t)a.s.count * a.v_heads * ((a.v_dim / 16 + 1) / 2);
     if (a.s.n <= DELTA_FEW || blocks > 0xFFFFFFull) return run_step(c, type, a);
+    const uint64_t least = std::min<uint64_t>(pl.at_once, 16);
     uint64_t n = pl.at_once;
-    if (pl.bytes(n) > c->part_bytes && grow_part(c, pl.bytes(n), true) != OKF_OK) {
-        n = c->part_bytes > pl.carry ? std::min((c->part_bytes - pl.carry) / pl.per_chunk, n) : 0;
-        if (n < std::min<uint64_t>(pl.at_once, 16)) return run_step(c, type, a);
+    while (pl.bytes(n) > c->part_bytes && grow_part(c, pl.bytes(n), true) != OKF_OK) {  // (what there is, or a quarter as much)
+        const uint64_t fit = c->part_bytes > pl.carry ? (c->part_bytes - pl.carry) / pl.per_chunk : 0;
+        if (fit < least && n / 4 < least) return run_step(c, type, a);
+        n = fit < least ? n / 4 : std::min(fit, n);
     }
     note_capture(c, false, true, false);
     float *carry = c->part;
@@ -244,7 +256,10 @@ int okf_conv_rows(okf_ctx *c, const okf_conv *p, const okf_state_seqs *s) {
     const uint64_t gy = (p->channels + per - 1) / per;
     if (gy > 65535 || items * gy > 0xFFFFFFull) return OKF_E_SHAPE;  // (a grid of less than 2^32 threads)
     if (!rows_apart(p->x, a.xs * size, (uint64_t)p->channels * size, s->n, p->y, a.ys * size, (uint64_t)p->channels * size, s->n)) return OKF_E_ARG;
-    if (!states_apart(s, (uint64_t)(p->width - 1) * p->channels * size)) return OKF_E_ARG;
+    const uint64_t each = (uint64_t)(p->width - 1) * p->channels * size, row = (uint64_t)p->channels * size;
+    if (!states_apart(s, each) || !state_apart(s->state_out, s, each, p->x, a.xs * size, row) ||
+        !state_apart(s->state_out, s, each, p->y, a.ys * size, row) || !state_apart(s->state_in, s, each, p->y, a.ys * size, row))
+        return OKF_E_ARG;
     if ((st = begin(c))) return st;
     const dim3 grid((uint32_t)items, (uint32_t)gy);
     with_type(p->type, [&](auto t) {

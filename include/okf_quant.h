@@ -423,11 +423,12 @@ typedef struct {
 int okf_norm_rope_rows(okf_ctx *ctx, const okf_norm_rope *r);
 
 /* Packed sequences that carry a state: sequence s has the rows [start[s], start[s + 1])
- * (starts that leave [0, n] or decrease are clamped) and the state slot[s] of `slots`
+ * (starts that leave [0, n] or decrease are clamped: nothing outside is touched; of sequences that
+ * overlap then some may be left out) and the state slot[s] of `slots`
  * (slot NULL: s).  It begins from state_in's, or from zeros where state_in is NULL, and
  * what it leaves goes to state_out's, where that is not NULL; a sequence without rows
- * leaves its state as it began.  state_out may be state_in; it may not overlap it in any other way
- * (OKF_E_ARG).  A slot outside [0, slots) begins from zeros and is not kept; two
+ * leaves its state as it began.  state_out may be state_in; it may not overlap it in any other way, nor the rows
+ * that the call reads, and neither of them those that it writes (OKF_E_ARG).  A slot outside [0, slots) begins from zeros and is not kept; two
  * sequences may share a slot only to begin from it (state_out NULL), else what is left
  * there is either's or a mixture.  Slots of no sequence stay as they are. */
 typedef struct {

@@ -31,7 +31,8 @@ def detached():
     ({"strides": (9, 0)}, ok.OKF_E_SHAPE), ({"strides": (0, 2 ** 41)}, ok.OKF_E_SHAPE), ({"channels": 2 ** 32 - 1, "n": 10 ** 6}, ok.OKF_E_SHAPE),
     ({"y": FAKE}, ok.OKF_E_ARG), ({"y": FAKE + 40}, ok.OKF_E_ARG), ({"y": FAKE + 40, "strides": (20, 20)}, ok.OKF_E_NODEV),
     ({"state_in": FAR, "state_out": FAR}, ok.OKF_E_NODEV), ({"state_in": FAR, "state_out": FAR + 120}, ok.OKF_E_ARG),
-    ({"state_in": FAR, "state_out": FAR + 240}, ok.OKF_E_NODEV)])
+    ({"state_in": FAR, "state_out": FAR + 240}, ok.OKF_E_NODEV), ({"state_out": FAKE}, ok.OKF_E_ARG), ({"state_out": FAKE << 4}, ok.OKF_E_ARG),
+    ({"state_in": FAKE << 4}, ok.OKF_E_ARG), ({"state_in": FAKE}, ok.OKF_E_NODEV)])
 def test_refusals(detached, over, status):
     a = dict(x=FAKE, w=FAKE, y=FAKE << 4, start=FAKE, seqs=2, n=7, channels=10, width=4)
     fails(lambda: detached.conv(**{**a, **over}), status)

@@ -50,7 +50,9 @@ def detached():
     ({"v": FAKE + 1024, "k": FAKE + 512, "out": FAKE + 3072, "strides": (1280,) * 4}, ok.OKF_E_NODEV),
     ({"v": FAKE + 1024, "k": FAKE + 512, "out": FAKE + 3056, "strides": (1280,) * 4}, ok.OKF_E_ARG),
     ({"state_in": FAR, "state_out": FAR}, ok.OKF_E_NODEV), ({"state_in": FAR, "state_out": FAR + 131072}, ok.OKF_E_ARG),
-    ({"state_in": FAR, "state_out": FAR + 262144}, ok.OKF_E_NODEV)])
+    ({"state_in": FAR, "state_out": FAR + 262144}, ok.OKF_E_NODEV), ({"state_out": FAKE * 32}, ok.OKF_E_ARG), ({"state_in": FAKE * 32}, ok.OKF_E_ARG),
+    ({"state_out": FAKE}, ok.OKF_E_ARG), ({"state_out": FAKE * 2}, ok.OKF_E_ARG), ({"state_out": FAKE * 4}, ok.OKF_E_ARG),
+    ({"state_out": FAKE * 8}, ok.OKF_E_ARG), ({"state_out": FAKE * 16}, ok.OKF_E_ARG), ({"state_in": FAKE * 4}, ok.OKF_E_NODEV)])
 def test_refusals(detached, form, over, status):
     a = dict(q=FAKE, k=FAKE * 2, v=FAKE * 4, g=FAKE * 8, beta=FAKE * 16, out=FAKE * 32, start=FAKE, seqs=2, n=7, k_heads=2, v_heads=4, k_dim=64,
              v_dim=128)

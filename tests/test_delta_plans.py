@@ -70,6 +70,15 @@ def test_scratch_that_may_not_grow(fake):
     assert r[2]["status"] == 0 and r[2]["launches"][0]["name"] == "delta_prepare_kernel" and r[2]["allocs"] == r[1]["allocs"]
 
 
+def test_scratch_that_cannot_be_had(fake):
+    """A device without room for the chunks: fewer of them, or token by token, and no error."""
+    call = ["delta", "prompt", "f32", 3200, 1, 2, 4, 64, 64]
+    r = fakehip_delta.run(fake, [["fail_above", 4000], call, call])  # (101 chunks are 12 MB, a quarter of them 3)
+    assert [s["status"] for s in r] == [0] * 3 and len(r[1]["launches"]) == 10 and r[2]["launches"] == r[1]["launches"]
+    r = fakehip_delta.run(fake, [["fail_above", 1], call, ["delta", "step", "f32", 3200, 1, 2, 4, 64, 64]])
+    assert [s["status"] for s in r] == [0] * 3 and r[1]["launches"] == r[2]["launches"]
+
+
 @pytest.mark.parametrize("seqs", [1, 5, 30])
 def test_few_rows_go_token_by_token(fake, seqs):
     r = fakehip_delta.run(fake, [["delta", "prompt", "bf16", n, seqs, 2, 4, 64, 64] for n in (1, 16, 17)] + [["delta", "step", "bf16", 16, seqs, 2, 4, 64, 64]])
