@@ -1,16 +1,15 @@
 // okf_conv.h -- the short causal convolution of each channel over packed sequences with
 // their states (okf_conv_rows): y[t] = act(b + sum_j w[j] x[t - W + 1 + j]).
 //
-// Bound by memory: a value is read once (the W - 1 rows in front of a block of CV_T once
-// more) and written once, 2 W + 4 operations for each.  7036 rows of 10240 bf16 channels, width 4, SiLU: 80 us, 3.7 TB/s
+// Bound by memory: a value is read once (the W - 1 rows in front of a thread's first once
+// more) and written once, 2 W + 4 operations for each.  7036 rows of 10240 bf16 channels, width 4, SiLU: 77 us, 3.8 TB/s
 // in and out; the vector units are half busy there, with conversions, products and SiLU, and the waits are what is left.
-// 32 sequences of one fp32 row: 5.4 us, the search for the sequence and two loads behind each other.
+// 32 sequences of one fp32 row: 5.4 us, the search for the sequence and two loads behind each other.  More than two wavefronts a SIMD fit but for 16-bit
+// types at widths from 6 (width 8 bf16, held to two: 512 rows 15.6 us for 18.5).
 #pragma once
 #include "okf_kv_seqs.h"
 
 namespace okf {
-
-constexpr uint32_t CV_T = 32;  // rows a thread goes through
 
 // Packed sequences and their states, as kernels take them.
 struct StateSeqs {
@@ -28,7 +27,7 @@ struct ConvArgs {
     void *y, *so;
     const float *w, *b;
     uint64_t xs, ys;
-    uint32_t channels, silu;
+    uint32_t channels, silu, rows;  // rows: that a thread goes through
     StateSeqs s;
 };
 
@@ -39,21 +38,21 @@ __device__ __forceinline__ float cv_silu(float x) {
     return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.4426950408889634f));
 }
 
-// A thread takes V channels (a 16-byte piece, or one) through up to CV_T rows of a sequence with the
+// A thread takes V channels (a 16-byte piece, or one) through up to `rows` rows of a sequence with the
 // last W - 1 rows in registers.  The thread of a sequence's first rows has read its
 // state before it writes what the sequence leaves, so that it may go to the same
 // place.
 template <class T, int W, int V>
-__global__ __launch_bounds__(256) void conv_kernel(const ConvArgs a) {
+__global__ __launch_bounds__(256, 2) void conv_kernel(const ConvArgs a) {
     typedef T vec __attribute__((ext_vector_type(V)));
     const SeqItem it = kv_find(blockIdx.x, a.s.count, [&](uint32_t s) {
         const uint2 r = kv_rows(a.s.start, s, a.s.n);
-        return max((r.y - r.x + CV_T - 1) / CV_T, 1u);
+        return max((r.y - r.x + a.rows - 1) / a.rows, 1u);
     });
     const uint32_t c = (blockIdx.y * 256 + threadIdx.x) * V;
     if (it.seq >= a.s.count || c >= a.channels) return;
     const uint2 r = kv_rows(a.s.start, it.seq, a.s.n);
-    const uint32_t first = r.x + it.at * CV_T, last = min(first + CV_T, r.y);
+    const uint32_t first = r.x + it.at * a.rows, last = min(first + a.rows, r.y);
     if (it.at && first >= r.y) return;  // (not with starts that rise)
     const int64_t slot = a.s.state(it.seq);
     const T *x = (const T *)a.x + c;
@@ -93,8 +92,8 @@ __global__ __launch_bounds__(256) void conv_kernel(const ConvArgs a) {
             *(vec *)(so + (uint64_t)j * a.channels) = v;
         }
     }
-    // (four rows on their way at a time)
-    constexpr uint32_t AHEAD = 4;
+    // (rows on their way at a time: 8 for 4 took 7036 bf16 rows of 10240 channels from 80 us to 77)
+    constexpr uint32_t AHEAD = W * V <= 32 ? 8 : 4;
     for (uint32_t t = first; t < last; t += AHEAD) {
         vec in[AHEAD];
 #pragma unroll

@@ -242,7 +242,7 @@ int okf_conv_rows(okf_ctx *c, const okf_conv *p, const okf_state_seqs *s) {
     if (!attn_type(p->type)) return OKF_E_TYPE;
     if (!p->channels || p->width < 2 || p->width > 8) return OKF_E_SHAPE;
     const uint32_t size = p->type == F32 ? 4 : 2, V = 16 / size;
-    ConvArgs a{p->x, s->state_in, p->y, s->state_out, p->w, p->bias, p->x_stride, p->y_stride, p->channels, (uint32_t)(p->silu != 0), seqs_of(s)};
+    ConvArgs a{p->x, s->state_in, p->y, s->state_out, p->w, p->bias, p->x_stride, p->y_stride, p->channels, (uint32_t)(p->silu != 0), 0, seqs_of(s)};
     for (uint64_t *r : {&a.xs, &a.ys}) {
         if (!*r) *r = p->channels;
         if (*r < p->channels || *r > 1ull << 40) return OKF_E_SHAPE;
@@ -252,8 +252,12 @@ int okf_conv_rows(okf_ctx *c, const okf_conv *p, const okf_state_seqs *s) {
     // 16-byte pieces where every row begins and ends with a whole one
     const bool wide = p->channels % V == 0 && a.xs % V == 0 && a.ys % V == 0 && aligned16(p->x) && aligned16(p->y) && aligned16(s->state_in) &&
                       aligned16(s->state_out);
-    const uint64_t items = std::min<uint64_t>(s->n, s->n / CV_T + s->seqs) + s->seqs, per = 256ull * (wide ? V : 1);
-    const uint64_t gy = (p->channels + per - 1) / per;
+    const uint64_t per = 256ull * (wide ? V : 1), gy = (p->channels + per - 1) / per;
+    // rows a thread: two workgroups a CU or more, in whole groups of 8 up to 32 (10240 bf16 channels: 64 rows 7.5 us by 8 and
+    // 13.6 by 32, 2000 21.9 and 23.5, by 24 20.3, 16000 162 and 142, by 64 145)
+    const uint64_t few = 16ull * (c ? c->cus : 256);
+    a.rows = (uint32_t)std::min<uint64_t>((s->n * gy + few - 1) / few, 4) * 8;
+    const uint64_t items = std::min<uint64_t>(s->n, s->n / a.rows + s->seqs) + s->seqs;
     if (gy > 65535 || items * gy > 0xFFFFFFull) return OKF_E_SHAPE;  // (a grid of less than 2^32 threads)
     if (!rows_apart(p->x, a.xs * size, (uint64_t)p->channels * size, s->n, p->y, a.ys * size, (uint64_t)p->channels * size, s->n)) return OKF_E_ARG;
     const uint64_t each = (uint64_t)(p->width - 1) * p->channels * size, row = (uint64_t)p->channels * size;

@@ -86,6 +86,15 @@ def test_conv(enc, t, C, W, lens):
 
 @gpu
 @pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("lens", [[4000], [5001, 0, 17], [3000, 1, 6003], [7, 12999, 33], [20000]])
+def test_long(enc, t, lens):
+    """Sums of rows from which a thread goes through 8, 16, 24 and 32 of them."""
+    check(enc, t, 40, 4, lens)
+    check(enc, t, 17, 3, lens, inplace=True)
+
+
+@gpu
+@pytest.mark.parametrize("t", ["f32", "bf16"])
 def test_slots(enc, t):
     """States anywhere in a pool; slots outside it begin from zeros and are not kept."""
     check(enc, t, 64, 4, [3, 1, 0, 40], slot=[6, 0, 3, 2], slots=8)
