@@ -4,8 +4,7 @@
 // Bound by memory: a value is read once (the W - 1 rows in front of a thread's first once
 // more) and written once, 2 W + 4 operations for each.  7036 rows of 10240 bf16 channels, width 4, SiLU: 77 us, 3.8 TB/s
 // in and out; the vector units are half busy there, with conversions, products and SiLU, and the waits are what is left.
-// 32 sequences of one fp32 row: 5.4 us, the search for the sequence and two loads behind each other.  More than two wavefronts a SIMD fit but for 16-bit
-// types at widths from 6 (width 8 bf16, held to two: 512 rows 15.6 us for 18.5).
+// 32 sequences of one fp32 row: 5.4 us, the search for the sequence and two loads behind each other.
 #pragma once
 #include "okf_kv_seqs.h"
 
@@ -42,6 +41,7 @@ __device__ __forceinline__ float cv_silu(float x) {
 // last W - 1 rows in registers.  The thread of a sequence's first rows has read its
 // state before it writes what the sequence leaves, so that it may go to the same
 // place.
+// (Two wavefronts a SIMD at least: bf16 at width 8 has one without that, 512 rows 18.5 us for 15.6.)
 template <class T, int W, int V>
 __global__ __launch_bounds__(256, 2) void conv_kernel(const ConvArgs a) {
     typedef T vec __attribute__((ext_vector_type(V)));
