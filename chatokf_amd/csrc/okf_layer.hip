@@ -214,7 +214,9 @@ int okf_norm_rope_rows(okf_ctx *c, const okf_norm_rope *p) {
     a.tq = (p->heads + G - 1) / G;
     a.tk = (kv + G - 1) / G;
     const uint32_t tasks = a.tq + a.tk;
-    a.per = std::max(1u, (uint32_t)std::min<uint64_t>(tasks, (uint64_t)p->n * tasks / (16 * c->cus)));
+    // tasks a wavefront: as many as leave 32 wavefronts a CU (4943 rows of 16 + 4 f16 heads of 256: 27.5 us, with 16 or 64
+    // wavefronts 29.6 and 32.8; 8192 rows of 40 + 8 bf16 heads of 128 43.3, 43.2 and 44.5)
+    a.per = std::max(1u, (uint32_t)std::min<uint64_t>(tasks, (uint64_t)p->n * tasks / (32 * c->cus)));
     a.wpr = (tasks + a.per - 1) / a.per;
     // (a grid of less than 2^32 threads; where rows are left a wavefront takes the next)
     const uint64_t waves = std::min<uint64_t>((uint64_t)p->n * a.wpr, (uint64_t)((1u << 22) / a.wpr + 1) * a.wpr);
@@ -257,7 +259,9 @@ int okf_conv_rows(okf_ctx *c, const okf_conv *p, const okf_state_seqs *s) {
     // 13.6 by 32, 2000 21.9 and 23.5, by 24 20.3, 16000 162 and 142, by 64 145)
     const uint64_t few = 16ull * (c ? c->cus : 256);
     a.rows = (uint32_t)std::min<uint64_t>((s->n * gy + few - 1) / few, 4) * 8;
-    const uint64_t items = std::min<uint64_t>(s->n, s->n / a.rows + s->seqs) + s->seqs;
+    auto count = [&] { return std::min<uint64_t>(s->n, s->n / a.rows + s->seqs) + s->seqs; };
+    while (count() * gy > 0xFFFFFFull && a.rows < 1u << 16) a.rows *= 2;
+    const uint64_t items = count();
     if (gy > 65535 || items * gy > 0xFFFFFFull) return OKF_E_SHAPE;  // (a grid of less than 2^32 threads)
     if (!rows_apart(p->x, a.xs * size, (uint64_t)p->channels * size, s->n, p->y, a.ys * size, (uint64_t)p->channels * size, s->n)) return OKF_E_ARG;
     const uint64_t each = (uint64_t)(p->width - 1) * p->channels * size, row = (uint64_t)p->channels * size;

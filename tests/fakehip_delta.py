@@ -20,6 +20,10 @@ class Child(fakehip._Child):
         P = self.P
         call(P, P, P, P, P, P << 32, P, seqs, n, k_heads, v_heads, k_dim, v_dim, type=self.ok.BY_NAME[t])
 
+    def conv(self, t, n, seqs, channels, width):
+        P = self.P
+        self.enc.conv(P, P, P << 32, P, seqs, n, channels, width, type=self.ok.BY_NAME[t])
+
     def delta_reserve(self, t, n, seqs, k_heads, v_heads, k_dim, v_dim):
         self.enc.delta_reserve(n, seqs, k_heads, v_heads, k_dim, v_dim, self.ok.BY_NAME[t])
 

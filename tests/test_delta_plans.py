@@ -99,6 +99,17 @@ def test_step_plan(fake, seqs, VH, DK, DV, args, grid):
     assert (x["name"], x["args"], x["grid"][0]) == ("delta_step_kernel", args, grid)
 
 
+@pytest.mark.parametrize("t,n,seqs,C,rows,wide", [("f32", 1, 1, 10240, 8, 4), ("bf16", 512, 1, 10240, 8, 8), ("bf16", 1000, 3, 10240, 16, 8),
+                                                  ("bf16", 2000, 1, 10240, 24, 8), ("bf16", 7036, 4, 10240, 32, 8), ("f32", 409, 2, 10240, 8, 4),
+                                                  ("f16", 500, 1, 2047, 8, 1), ("f32", 2 ** 31 - 256, 1, 16, 256, 4)])
+def test_conv_plan(fake, t, n, seqs, C, rows, wide):
+    """Rows a thread by the workgroups that they leave; 16 bytes of channels where rows begin and end with whole ones."""
+    (r,) = fakehip_delta.run(fake, [["conv", t, n, seqs, C, 4]])
+    (x,) = r["launches"]
+    assert (x["name"], x["args"], x["grid"][1]) == ("conv_kernel", [4, wide], -(-C // (256 * wide)))
+    assert x["grid"][0] == min(n, n // rows + seqs) + seqs
+
+
 # ------------------------------------------------------------------ on the GPU
 @gpu
 @pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
