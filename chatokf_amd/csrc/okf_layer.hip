@@ -44,6 +44,18 @@ int rope_freqs(const okf_rope &r, double *f, float &mag) {
 // Bytes of a row whose heads stand `head` values apart.
 uint64_t row_bytes(uint32_t heads, uint64_t head, uint32_t dim, uint32_t size) { return ((heads - 1) * head + dim) * size; }
 
+// Whether two heads of n rows, `row` values apart, of `heads` heads, `head` apart, share any of their dim values.  Rows
+// of one head do not (row >= dim), nor heads of one row; head h of a row starts h * head behind the row's first
+// head, and of those only the nearest two, one on either side, can be less than dim away.
+bool heads_meet(uint64_t row, uint64_t head, uint32_t n, uint32_t heads, uint32_t dim) {
+    if (row >= (heads - 1) * head + dim || head >= (unsigned __int128)(n - 1) * row + dim) return false;
+    for (uint32_t h = 1; h < heads; h++) {
+        const uint64_t r = h * head / row, past = h * head % row;
+        if ((r < n && past < dim) || (r + 1 < n && row - past < dim)) return true;
+    }
+    return false;
+}
+
 template <class T, int L>
 void launch_rope(okf_ctx *c, const RopeArgs &a, bool cross, uint32_t grid) {
     if (cross) hipLaunchKernelGGL((norm_rope_kernel<T, L, true>), dim3(grid), dim3(RP_NT), 0, c->stream, a);
@@ -204,6 +216,7 @@ int okf_norm_rope_rows(okf_ctx *c, const okf_norm_rope *p) {
     };
     auto same = [](const Rows &x, const Rows &y) { return x.p == y.p && x.stride == y.stride && x.head == y.head; };
     if ((!same(q, qo) && !apart(q, qo)) || (!same(k, ko) && !apart(k, ko)) || !apart(q, ko) || !apart(k, qo) || !apart(qo, ko)) return OKF_E_ARG;
+    if (heads_meet(a.qos, a.qoh, p->n, p->heads, p->dim) || (kv && heads_meet(a.kos, a.koh, p->n, kv, p->dim))) return OKF_E_ARG;
     int st = rope_freqs(r, a.f, a.mag);
     if (st) return st;
     if ((st = begin(c))) return st;

@@ -404,8 +404,8 @@ typedef struct {
  * fp32 inside, rounded once to `type`.  k may be NULL (heads of one kind).  With norms
  * of dim^-0.5 and eps / dim for eps this is x / sqrt(sum(x^2) + eps), the delta rule's
  * unit vectors.  q_out may be q and k_out k, with the same strides; other overlaps of
- * outputs with inputs or each other are an OKF_E_ARG (so are ranges that lie inside each
- * other's rows with row strides that differ). */
+ * outputs with q and k, each other or themselves (heads that share values) are an OKF_E_ARG (so are
+ * ranges that lie inside each other's rows with row strides that differ). */
 typedef struct {
     const void *q, *k;              /* rows of heads x dim / kv_heads x dim values */
     void *q_out, *k_out;
