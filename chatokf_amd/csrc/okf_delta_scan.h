@@ -11,14 +11,17 @@
 // sequence's chunks one behind the other with the state in registers.
 //
 // Precision: every product has fp32's.  An fp32 value is three bf16 parts (x = x0 + x1 + x2
-// exactly, each the next eight bits), f16 inputs are two, bf16 one; of the products of parts those
-// below 2^-24 of the whole are left out.  G and its differences are in 64 bits, so that
+// exactly, each what is left rounded to nearest), f16 inputs are two, bf16 one; of the products of parts those that
+// come to less than 2^-24 of the whole, of either sign, are left out: |x1| <= 2^-8 and |x2| <= 2^-17 of a power of two
+// that |x| reaches, so x1 y2 + x2 y1 + x2 y2.  (Parts that are cut off have the sign of x, and what is left out
+// reaches 2^-21, 0.7 2^-24 on average.)  G and its differences are in 64 bits, so that
 // decays far apart keep their ratios.  (I + A)^-1 comes from forward substitution, which
 // is as stable as the recurrence; powers of A are not.
 //
 // Where something is not finite, 0 times it in the places that a mask or the order of tokens
 // leaves out would spread it to earlier tokens: columns whose corrections show any are gone through
-// again token by token.  (A chunk whose queries are not finite has its T spoilt, so that it shows.)
+// again token by token.  (A chunk whose queries are not finite has its T spoilt, so that it shows.  Values
+// from 2^127 on count as not finite: those next to the type's end have no first part.)
 #pragma once
 #include <utility>
 
@@ -60,6 +63,15 @@ __device__ __forceinline__ uint32_t dl_before(const StateSeqs &s, uint32_t seq) 
     return sum;
 }
 
+// Two floats as bf16, rounded to nearest even, a in the lower half; and the lower's and the upper's value.
+typedef __bf16 bf16x2d __attribute__((ext_vector_type(2)));
+typedef float floatx2d __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t dl_round(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((floatx2d{a, b}), bf16x2d));
+}
+__device__ __forceinline__ float dl_lower(uint32_t p) { return __uint_as_float(p << 16); }
+__device__ __forceinline__ float dl_upper(uint32_t p) { return __uint_as_float(p & 0xFFFF0000u); }
+
 // Eight floats -> NP bf16 parts of each.
 template <int NP>
 __device__ __forceinline__ void dl_split(const float (&x)[8], bf16x8d (&p)[NP]) {
@@ -69,17 +81,16 @@ __device__ __forceinline__ void dl_split(const float (&x)[8], bf16x8d (&p)[NP]) 
         float a = x[2 * j], b = x[2 * j + 1];
 #pragma unroll
         for (int n = 0; n < NP; n++) {
-            const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
-            out[n][j] = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
-            if (n < NP - 1) a -= __uint_as_float(ua & 0xFFFF0000u), b -= __uint_as_float(ub & 0xFFFF0000u);
+            out[n][j] = dl_round(a, b);
+            if (n < NP - 1) a -= dl_lower(out[n][j]), b -= dl_upper(out[n][j]);
         }
     }
 #pragma unroll
     for (int n = 0; n < NP; n++) p[n] = __builtin_bit_cast(bf16x8d, out[n]);
 }
 
-// The parts of two results below each other, as the B operand of the next product, step by step: dl_top takes
-// the first eight bits of every value, what they leave is the value less them, for one of the four
+// The parts of two results below each other, as the B operand of the next product, step by step: dl_top rounds
+// every value to its first part, what that leaves is the value less it, for one of the four
 // values of both in dl_rest; or from the matrix cores, -1 times the part added to the value (exact: the
 // difference has fewer bits).
 struct DlMinus {
@@ -96,20 +107,22 @@ __device__ __forceinline__ bf16x8d dl_top(floatx4 x, floatx4 y) {
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const float a = j < 2 ? x[2 * j] : y[2 * j - 4], b = j < 2 ? x[2 * j + 1] : y[2 * j - 3];
-        p[j] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+        p[j] = dl_round(a, b);
     }
     return __builtin_bit_cast(bf16x8d, p);
 }
-__device__ __forceinline__ void dl_rest(floatx4 &x, floatx4 &y, int j) {
-    x[j] -= __uint_as_float(__float_as_uint(x[j]) & 0xFFFF0000u);
-    y[j] -= __uint_as_float(__float_as_uint(y[j]) & 0xFFFF0000u);
+__device__ __forceinline__ void dl_rest(floatx4 &x, floatx4 &y, bf16x8d part, int j) {
+    const u32x4 p = __builtin_bit_cast(u32x4, part);
+    const uint32_t px = p[j / 2], py = p[2 + j / 2];
+    x[j] -= j % 2 ? dl_upper(px) : dl_lower(px);
+    y[j] -= j % 2 ? dl_upper(py) : dl_lower(py);
 }
 __device__ __forceinline__ void dl_split(floatx4 x, floatx4 y, bf16x8d (&p)[3]) {
 #pragma unroll
     for (int n = 0; n < 3; n++) {
         p[n] = dl_top(x, y);
 #pragma unroll
-        for (int j = 0; n < 2 && j < 4; j++) dl_rest(x, y, j);
+        for (int j = 0; n < 2 && j < 4; j++) dl_rest(x, y, p[n], j);
     }
 }
 __device__ __forceinline__ floatx4 dl_mfma(bf16x8d a, bf16x8d b, floatx4 d) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, d, 0, 0, 0); }
@@ -187,11 +200,9 @@ typedef short shortx4d __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void dl_split4(floatx4 x, shortx4d (&p)[3]) {
 #pragma unroll
     for (int n = 0; n < 3; n++) {
-        const uint2 t = {__builtin_amdgcn_perm(__float_as_uint(x[1]), __float_as_uint(x[0]), 0x07060302u),
-                         __builtin_amdgcn_perm(__float_as_uint(x[3]), __float_as_uint(x[2]), 0x07060302u)};
+        const uint2 t = {dl_round(x[0], x[1]), dl_round(x[2], x[3])};
         p[n] = __builtin_bit_cast(shortx4d, t);
-#pragma unroll
-        for (int j = 0; j < 4; j++) x[j] -= __uint_as_float(__float_as_uint(x[j]) & 0xFFFF0000u);
+        x -= floatx4{dl_lower(t.x), dl_upper(t.x), dl_lower(t.y), dl_upper(t.y)};
     }
 }
 __device__ __forceinline__ floatx4 dl_mma16(floatx4 x, floatx4 y) {
@@ -357,7 +368,7 @@ __global__ __launch_bounds__(DP_NT) void delta_prepare_kernel(const ScanArgs p) 
 #pragma unroll
         for (int t = 0; t < 3; t++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) bad = fmaf(P[z][t][i], 0.0f, bad);
+            for (int i = 0; i < 4; i++) bad = fmaf(2 * P[z][t][i], 0.0f, bad);
         floatx4 lo = r11 * b0;
         if (__ballot(bad != bad)) lo[0] = __builtin_nanf("");
         bf16x8d *to = (bf16x8d *)vb(vh + z) + lane;
@@ -564,7 +575,7 @@ __global__ __launch_bounds__(DN_NT, (dl_two<T, KS>() ? 2 : 1)) void delta_scan_k
                                 top(st, 0);
                                 x[st][0] = S[2 * st], x[st][1] = S[2 * st + 1];
                             }
-                            if (i > 0) dl_rest(x[st][0], x[st][1], i - 1);
+                            if (i > 0) dl_rest(x[st][0], x[st][1], sp[st][0], i - 1);
                         }
                     });
             });
@@ -598,7 +609,7 @@ __global__ __launch_bounds__(DN_NT, (dl_two<T, KS>() ? 2 : 1)) void delta_scan_k
             u[0] = u[1] = floatx4{0, 0, 0, 0};
             auto rest = [&](int n) {
                 return [&, n](int i) {
-                    if (i < 4) dl_rest(v[0], v[1], i);
+                    if (i < 4) dl_rest(v[0], v[1], part[n - 1], i);
                     else part[n] = dl_top(v[0], v[1]);
                 };
             };
@@ -713,7 +724,7 @@ __global__ __launch_bounds__(DN_NT, (dl_two<T, KS>() ? 2 : 1)) void delta_scan_k
             bf16x8d part[3];
             dl_split(from.u[0][lane], from.u[1][lane], part);
 #pragma unroll
-            for (int j = 0; j < 8; j++) bad = fmaf(from.u[j / 4][lane][j % 4], 0.0f, bad);
+            for (int j = 0; j < 8; j++) bad = fmaf(2 * from.u[j / 4][lane][j % 4], 0.0f, bad);
 #pragma unroll
             for (int mt = 0; mt < 2; mt++) o[mt] = dl_mma(pp[mt], part, o[mt] * eg[mt]);
             fix();
