@@ -2,8 +2,9 @@
 // their states (okf_conv_rows): y[t] = act(b + sum_j w[j] x[t - W + 1 + j]).
 //
 // Bound by memory: a value is read once (the W - 1 rows in front of a thread's first once
-// more) and written once, 2 W + 4 operations for each.  7036 rows of 10240 bf16 channels, width 4, SiLU: 77 us, 3.8 TB/s
-// in and out; the vector units are half busy there, with conversions, products and SiLU, and the waits are what is left.
+// more) and written once, 2 W + 4 operations for each.  7036 rows of 10240 channels, width 4, SiLU: fp32 123 us, 4.7 TB/s in and
+// out; bf16 77 us, 3.8 TB/s: the vector units are busy for half of that, with conversions, products and SiLU, and wavefronts
+// wait for a third of it, since a group's loads begin only when the one before is used up, behind its stores.
 // 32 sequences of one fp32 row: 5.4 us, the search for the sequence and two loads behind each other.
 #pragma once
 #include "okf_kv_seqs.h"
@@ -41,7 +42,7 @@ __device__ __forceinline__ float cv_silu(float x) {
 // last W - 1 rows in registers.  The thread of a sequence's first rows has read its
 // state before it writes what the sequence leaves, so that it may go to the same
 // place.
-// (Two wavefronts a SIMD at least: bf16 at width 8 has one without that, 512 rows 18.5 us for 15.6.)
+// (Two wavefronts a SIMD at least: bf16 at width 8 has one without that, 512 rows 18.5 us for 15.6; with it a lane spills 20 bytes.)
 template <class T, int W, int V>
 __global__ __launch_bounds__(256, 2) void conv_kernel(const ConvArgs a) {
     typedef T vec __attribute__((ext_vector_type(V)));

@@ -225,7 +225,7 @@ constexpr uint32_t DP_ROW = 20;  // floats from a row of a 16 x 16 matrix in LDS
 // times the identity, whose result lies as an operand too.  (I + A)^-1 in 2 x 2 blocks of 16: those on the diagonal by
 // substitution from the right (t_j = delta_ij - sum_l>j t_l A_lj), both of both heads at once, a row a lane; the lower one
 // as -T22 (A21 T11).  Many chunks are bound by memory: 8192 tokens of 16 key and 48 value heads of 128, bf16, 76 us for 128 MB in
-// and 255 MB of scratch out; few by the chain itself, 15 us (K, Q and K^T laid out by other wavefronts: 14, many chunks 88 for 77).
+// and 255 MB of scratch out (fp32 113, 456 MB out); few by the chain itself, 15 us (K, Q and K^T laid out by other wavefronts: 14, many chunks 88 for 77).
 template <class T, int KS>
 __global__ __launch_bounds__(DP_NT) void delta_prepare_kernel(const ScanArgs p) {
     constexpr int NP = dl_parts<T>();
@@ -447,7 +447,8 @@ constexpr bool dl_two() { return KS * dl_parts<T>() <= 6 && KS < 6; }
 // Bound by the first wavefront's chain, chunk after chunk: 8192 tokens of 48 heads of 128 x 128, bf16, 366 us; without
 // any loads 280, 1.1 us a chunk of 68 matrix and some 250 vector instructions in order.  Tried and not faster: the operands brought to LDS once
 // for both halves (434 us, with Q S in the first wavefront then), what a part leaves of a value always by the
-// matrix cores (363).
+// matrix cores (363).  fp32, three parts of K, Q and K^T for one: 116 matrix instructions a chunk in that chain and three times
+// the operands, 758 us; f16 597.
 template <class T, int KS>
 __global__ __launch_bounds__(DN_NT, (dl_two<T, KS>() ? 2 : 1)) void delta_scan_kernel(const ScanArgs p) {
     constexpr int NP = dl_parts<T>();

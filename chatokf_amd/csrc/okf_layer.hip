@@ -135,8 +135,10 @@ int run_step(okf_ctx *c, int32_t type, const DeltaArgs &a) {
 // DELTA_WORK bytes, a grid of less than 2^32 threads), and the bytes of a chunk and of two states
 // that go from one launch to the next.
 constexpr uint64_t DELTA_WORK = 512ull << 20;
-// Prompts of no more rows go token by token: 48 heads of 128 x 128 take 12 us for 8 fp32 tokens and 21 for 16,
-// 9.5 and 16 for bf16 ones, two launches of chunks 22 and 16.
+// Prompts of no more rows go token by token.  One sequence's 16 tokens by steps, and 17 in chunks (us): 48 heads of 128 x 128
+// 20.9 and 22 fp32, 15.9 and 17 bf16; 24 of 96 x 208 bf16 14.0 and 15.1; 4 of 64 x 64 fp32 11.7 and 14.7; 32 of 256 x 256 21.3 and
+// 37 fp32, 22.2 and 25.1 bf16.  (The call's rows are counted: 8 sequences of 4 fp32 tokens, 48 heads, take 67 in chunks and
+// 12.8 by okf_delta_step, which is for such calls.)
 constexpr uint32_t DELTA_FEW = 16;
 struct DeltaPlan {
     uint64_t chunks, at_once, per_chunk, carry;
@@ -268,8 +270,9 @@ int okf_conv_rows(okf_ctx *c, const okf_conv *p, const okf_state_seqs *s) {
     const bool wide = p->channels % V == 0 && a.xs % V == 0 && a.ys % V == 0 && aligned16(p->x) && aligned16(p->y) && aligned16(s->state_in) &&
                       aligned16(s->state_out);
     const uint64_t per = 256ull * (wide ? V : 1), gy = (p->channels + per - 1) / per;
-    // rows a thread: two workgroups a CU or more, in whole groups of 8 up to 32 (10240 bf16 channels: 64 rows 7.5 us by 8 and
-    // 13.6 by 32, 2000 21.9 and 23.5, by 24 20.3, 16000 162 and 142, by 64 145)
+    // rows a thread, in whole groups of 8 up to 32: more than 8 only where that leaves more than one workgroup a CU, two just
+    // before each step (10240 bf16 channels: 64 rows 7.5 us by 8 and 13.6 by 32, 2000 21.9 and 23.5, by 24 20.3, 16000 162
+    // and 142, by 64 145)
     const uint64_t few = 16ull * (c ? c->cus : 256);
     a.rows = (uint32_t)std::min<uint64_t>((s->n * gy + few - 1) / few, 4) * 8;
     auto count = [&] { return std::min<uint64_t>(s->n, s->n / a.rows + s->seqs) + s->seqs; };

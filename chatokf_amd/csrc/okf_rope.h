@@ -27,7 +27,7 @@ struct RopeArgs {
 };
 
 // cos and sin of 2 pi t: t less the nearest quarter is at most 1/8, where the series of
-// both in x = 2 pi t, |x| <= pi / 4, are left off below 1e-10; the quarter swaps and signs them.
+// both in x = 2 pi t, |x| <= pi / 4, are left off below 1.2e-10; the quarter swaps and signs them.
 __device__ __forceinline__ float2 rp_turn(double t) {
     t -= rint(t);
     const double q = rint(4 * t);

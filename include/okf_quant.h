@@ -401,7 +401,8 @@ typedef struct {
 /* Norms and rotation of queries and keys, head by head, in one pass: for each of the n
  * rows and each head, y = x * norm / sqrt(mean(x^2) + eps) where that norm is not NULL,
  * then the rotation of y's first rot dimensions by the row's position; the others stay.
- * fp32 inside, rounded once to `type`.  k may be NULL (heads of one kind).  With norms
+ * fp32 inside, rounded once to `type`; squares are summed there too, so that a head whose mean(x^2) + eps
+ * is below 2^-126 or past fp32's largest number has no meaningful norm.  k may be NULL (heads of one kind).  With norms
  * of dim^-0.5 and eps / dim for eps this is x / sqrt(sum(x^2) + eps), the delta rule's
  * unit vectors.  q_out may be q and k_out k, with the same strides; other overlaps of
  * outputs with q and k, each other or themselves (heads that share values) are an OKF_E_ARG (so are
@@ -419,7 +420,8 @@ typedef struct {
     const int32_t *pos;             /* device memory, n positions (any int32); may be NULL with rot = 0 */
     okf_rope rope;
 } okf_norm_rope;
-/* Pointers are 16-byte aligned (pos, norms and div 4), strides whole multiples of 16 bytes. */
+/* Pointers are 16-byte aligned (pos, norms and div 4), strides whole multiples of 16 bytes.  pos, norms and div
+ * may not lie in the outputs (not checked). */
 int okf_norm_rope_rows(okf_ctx *ctx, const okf_norm_rope *r);
 
 /* Packed sequences that carry a state: sequence s has the rows [start[s], start[s + 1])
@@ -428,7 +430,8 @@ int okf_norm_rope_rows(okf_ctx *ctx, const okf_norm_rope *r);
  * (slot NULL: s).  It begins from state_in's, or from zeros where state_in is NULL, and
  * what it leaves goes to state_out's, where that is not NULL; a sequence without rows
  * leaves its state as it began.  state_out may be state_in; it may not overlap it in any other way, nor the rows
- * that the call reads, and neither of them those that it writes (OKF_E_ARG).  A slot outside [0, slots) begins from zeros and is not kept; two
+ * that the call reads, and neither of them those that it writes (OKF_E_ARG); nor may start and slot lie in
+ * anything that the call writes (not checked).  A slot outside [0, slots) begins from zeros and is not kept; two
  * sequences may share a slot only to begin from it (state_out NULL), else what is left
  * there is either's or a mixture.  Slots of no sequence stay as they are. */
 typedef struct {
@@ -443,7 +446,8 @@ typedef struct {
  * j < width of w[c][j] x[t - width + 1 + j][c]), act the identity or silu(x) = x / (1 +
  * exp(-x)); rows before a sequence's first are its state's, [slot][width - 1][channels]
  * of `type`, the oldest first.  fp32 inside, y rounded once; states are copied.  y may not
- * overlap x (OKF_E_ARG). */
+ * overlap x (OKF_E_ARG), nor w and bias lie in y or state_out (not checked).  seqs times the 256s of pieces in a
+ * row (of 16 bytes where rows, strides and pointers are whole ones, else of a channel) stays below some 2^23 (OKF_E_SHAPE). */
 typedef struct {
     const void *x;                  /* n rows of `channels` values */
     void *y;
@@ -461,7 +465,7 @@ int okf_conv_rows(okf_ctx *ctx, const okf_conv *a, const okf_state_seqs *s);
  * with the queries and keys of key head h / (v_heads / k_heads).  Keys of length about
  * one and beta in [0, 2] keep it stable; nothing here normalizes them (okf_norm_rope_rows).
  * g may be -inf: the state is cleared before the token.  All sums are in fp32 or with
- * fp32's precision, for values between 2^-100 and 2^100; o is rounded once. */
+ * fp32's precision, where values and the products of two of them lie between 2^-100 and 2^100; o is rounded once. */
 typedef struct {
     const void *q, *k, *v;          /* rows of k_heads x k_dim, k_heads x k_dim, v_heads x v_dim values */
     const float *g, *beta;          /* rows of v_heads values */
