@@ -27,7 +27,7 @@ def mean_bound(n):
 
 def numbers(rng, shape, t):
     x = (rng.uniform(1, 2, shape) * 2.0 ** rng.integers(-2, 3, shape) * rng.choice((-1, 1), shape)).astype(np.float32)
-    return x if t == "f32" else dev(x, TYPES[t]).float().cpu().numpy() if torch.cuda.is_available() else x
+    return torch.from_numpy(x).to(TYPES[t]).float().numpy()
 
 
 class Products:
